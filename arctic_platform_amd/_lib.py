@@ -14,7 +14,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libzorro_fca.so")
 CSRC_DIR = os.path.join(_HERE, "csrc")
 
-FCA_BF16, FCA_FP8_E4M3, FCA_F32 = 0, 1, 2
+FCA_BF16, FCA_FP8_E4M3, FCA_F32, FCA_FP8_E4M3_BLOCK = 0, 1, 2, 3
 FCA_MAX_LEVELS = 8
 FCA_STATIC_SCRATCH_BYTES = 48 << 20
 
@@ -36,6 +36,8 @@ EXPORTS = (
     "fca_decode_step_static",
     "fca_append_kv",
     "fca_gather_kv",
+    "fca_append_kv_block_scaled",
+    "fca_gather_kv_block_scaled",
     "fca_calibration_copy",
     "fca_time_next_attention",
     "fca_split_layout_ints",
@@ -179,6 +181,8 @@ def declare_signatures(lib: ctypes.CDLL) -> ctypes.CDLL:
     lib.fca_decode_step_static.argtypes = [P(FcaPlan), P(FcaTensors), VP, VP, I64, I64, I32, VP, VP]
     lib.fca_append_kv.argtypes = [VP, VP, I64, I64, I32, I32, I32, VP, VP, VP, I64, I64, I32, VP, VP, VP]
     lib.fca_gather_kv.argtypes = lib.fca_append_kv.argtypes
+    lib.fca_append_kv_block_scaled.argtypes = [VP, VP, I64, I64, I32, I32, I32, VP, VP, VP, I64, I64, I64, VP, VP]
+    lib.fca_gather_kv_block_scaled.argtypes = lib.fca_append_kv_block_scaled.argtypes
     lib.fca_calibration_copy.argtypes = [VP, VP, ctypes.c_size_t, VP]
     lib.fca_time_next_attention.argtypes = [VP, VP]
     F32 = ctypes.c_float

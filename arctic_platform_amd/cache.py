@@ -11,32 +11,62 @@ engine's attention backend, which is what this call replaces.
 
 from __future__ import annotations
 
+import contextlib
+
 import torch
 
 from . import _lib
 from .forest import _stream_ptr
-from .kv_layout import BLOCK_SIZE
+from .kv_layout import BLOCK_SIZE, block_scales_shape
 
 
-def gather_kv(kv_cache, slot_mapping, head_dim, k_scale=None, v_scale=None, out=None):
+def on_device(device):
+    """A launch goes to the current device: makes ``device`` that for a call on another one's tensors."""
+    if device.type != "cuda" or device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
+
+
+def check_block_scales(block_scales, kv_cache, k_scale, v_scale) -> None:
+    """The scale table of a block-scaled cache (``kv_layout.block_scales_shape``) against its cache."""
+    if kv_cache.dtype != torch.float8_e4m3fn:
+        raise TypeError(f"block_scales belong to a float8_e4m3fn cache, got {kv_cache.dtype}")
+    if k_scale is not None or v_scale is not None:
+        raise ValueError("a cache has either block_scales or per-head k_scale / v_scale")
+    want = block_scales_shape(kv_cache.shape[1], kv_cache.shape[2])
+    if block_scales.dtype != torch.float32 or tuple(block_scales.shape) != want or not block_scales.is_contiguous():
+        raise ValueError(f"block_scales must be a contiguous fp32 tensor of shape {list(want)}")
+    if block_scales.device != kv_cache.device:
+        raise ValueError(f"block_scales are on {block_scales.device}, the cache is on {kv_cache.device}")
+
+
+def gather_kv(kv_cache, slot_mapping, head_dim, k_scale=None, v_scale=None, out=None, block_scales=None):
     """The way back: bf16 ``(key, value)`` rows ``[T, Hkv, D]`` of the tokens at ``slot_mapping``
-    (fp8 caches times their scales: the values decode attention sees; negative slot = zeros)."""
+    (fp8 caches times their scales, per head or ``block_scales``: the values decode attention
+    sees; negative slot = zeros, and with ``block_scales`` a slot past the cache too)."""
     hkv = kv_cache.shape[2]
     t = slot_mapping.shape[0]
     if out is None:
         rows_dtype = torch.float32 if kv_cache.dtype == torch.float32 else torch.bfloat16
         out = tuple(torch.empty(t, hkv, head_dim, dtype=rows_dtype, device=kv_cache.device) for _ in range(2))
-    _cache_rows(True, out[0], out[1], kv_cache, slot_mapping, k_scale, v_scale)
+    _cache_rows(True, out[0], out[1], kv_cache, slot_mapping, k_scale, v_scale, block_scales)
     return out
 
 
-def append_kv(key, value, kv_cache, slot_mapping, k_scale=None, v_scale=None) -> None:
+def append_kv(key, value, kv_cache, slot_mapping, k_scale=None, v_scale=None, block_scales=None) -> None:
     """key, value: bf16 ``[T, Hkv, D]`` (float32 for a float32 cache); slot_mapping: int64 ``[T]``;
-    kv_cache as in kv_layout."""
-    _cache_rows(False, key, value, kv_cache, slot_mapping, k_scale, v_scale)
+    kv_cache as in kv_layout.
+
+    With ``block_scales`` (fp32 ``[num_blocks, Hkv, 2]``) the fp8 cache is block-scaled and its scales
+    are taken from the data: a block's scale is the smallest power of two that holds the call's
+    tokens of the block, or the one the block has if that is larger; where it grows, the block's
+    earlier codes are moved to it.  A token at offset 0 begins its block: what the block held
+    before, and its scale, are forgotten.  Slots past the cache are skipped like negative ones; of
+    two tokens with one slot the later is stored (``fca_append_kv_block_scaled``)."""
+    _cache_rows(False, key, value, kv_cache, slot_mapping, k_scale, v_scale, block_scales)
 
 
-def _cache_rows(gather, key, value, kv_cache, slot_mapping, k_scale, v_scale) -> None:
+def _cache_rows(gather, key, value, kv_cache, slot_mapping, k_scale, v_scale, block_scales=None) -> None:
     f32 = kv_cache.dtype == torch.float32
     rows_dtype = torch.float32 if f32 else torch.bfloat16
     if key.dtype != rows_dtype or value.dtype != rows_dtype or key.shape != value.shape or key.dim() != 3:
@@ -68,6 +98,19 @@ def _cache_rows(gather, key, value, kv_cache, slot_mapping, k_scale, v_scale) ->
         if sc is not None and (sc.dtype != torch.float32 or sc.shape != (hkv,) or not sc.is_contiguous()):
             raise ValueError(f"{name} must be a contiguous fp32 tensor of shape [{hkv}]")
     lib = _lib.load_library()
+    if block_scales is not None:
+        check_block_scales(block_scales, kv_cache, k_scale, v_scale)
+        if not key.device == value.device == kv_cache.device == slot_mapping.device:
+            raise ValueError("key, value, slot_mapping and the cache must be on one device")
+        with on_device(kv_cache.device):
+            _lib.check(
+                (lib.fca_gather_kv_block_scaled if gather else lib.fca_append_kv_block_scaled)(
+                    key.data_ptr(), value.data_ptr(), key.stride(0), key.stride(1), t, hkv, d, slot_mapping.data_ptr(),
+                    kv_cache.data_ptr(), kv_cache.data_ptr() + kv_cache.stride(0), kv_cache.stride(1), kv_cache.stride(2),
+                    kv_cache.shape[1], block_scales.data_ptr(), _stream_ptr(kv_cache.device),
+                )
+            )
+        return
     esz = kv_cache.element_size()
     _lib.check(
         (lib.fca_gather_kv if gather else lib.fca_append_kv)(

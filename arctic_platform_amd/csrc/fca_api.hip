@@ -5,6 +5,7 @@
 #include <cstring>
 #include <mutex>
 
+#include "fca_block_scales.h"
 #include "fca_common.h"
 
 namespace {
@@ -52,7 +53,9 @@ int check_plan(const fca_plan* p) {
   return FCA_OK;
 }
 
-int kv_elem_bytes(int kv_dtype) { return kv_dtype == FCA_FP8_E4M3 ? 1 : kv_dtype == FCA_F32 ? 4 : 2; }
+int kv_elem_bytes(int kv_dtype) {
+  return kv_dtype == FCA_FP8_E4M3 || kv_dtype == FCA_FP8_E4M3_BLOCK ? 1 : kv_dtype == FCA_F32 ? 4 : 2;
+}
 
 // f32_ok: the entry point has an fp32 path (fca_decode_step and fca_decode_step_static)
 int check_tensors(const fca_plan* p, const fca_tensors* t, bool f32_ok = false) {
@@ -66,6 +69,11 @@ int check_tensors(const fca_plan* p, const fca_tensors* t, bool f32_ok = false) 
       return fail(FCA_ERR_UNSUPPORTED, "the fp32 path takes head_dim 64 or 128, got %d", p->head_dim);
     if (p->rows_per_item != 32)
       return fail(FCA_ERR_UNSUPPORTED, "the fp32 path takes rows_per_item 32, got %d", p->rows_per_item);
+  } else if (t->kv_dtype == FCA_FP8_E4M3_BLOCK) {
+    if (!t->k_scale_dev || t->v_scale_dev || (reinterpret_cast<uintptr_t>(t->k_scale_dev) & 7))
+      return fail(FCA_ERR_INVALID_ARG,
+                  "a block-scaled cache takes its scale table in k_scale (8-byte aligned) and no v_scale");
+    if (!(t->softmax_scale > 0.f)) return fail(FCA_ERR_INVALID_ARG, "softmax_scale must be positive, got %g", (double)t->softmax_scale);
   } else if (t->kv_dtype != FCA_BF16 && t->kv_dtype != FCA_FP8_E4M3) {
     return fail(FCA_ERR_UNSUPPORTED, "kv_dtype %d is not supported (bf16, fp8 e4m3, or fp32 with an fp32 q)", t->kv_dtype);
   }
@@ -137,6 +145,8 @@ int run_attend(const fca_plan* p, const fca_tensors* t, void* meta, void* po, fl
   const fca::AttendParams a = attend_params(p, t, meta, po, pl, select);
   hipError_t e = t->kv_dtype == FCA_F32
                      ? fca::launch_attend_f32(a, *p, t->max_workgroups, static_cast<hipStream_t>(stream))
+                 : t->kv_dtype == FCA_FP8_E4M3_BLOCK
+                     ? fca::launch_attend_block(a, *p, t->max_workgroups, static_cast<hipStream_t>(stream))
                      : fca::launch_attend(a, *p, t->kv_dtype, t->max_workgroups, t->tile_buffers, static_cast<hipStream_t>(stream));
   return e == hipSuccess ? FCA_OK : hip_fail(e, "attention pass launch");
 }
@@ -189,7 +199,7 @@ int fca_workspace_bytes(const fca_plan* plan, size_t* meta_bytes, size_t* partia
 int fca_workspace_bytes_dtype(const fca_plan* plan, int32_t kv_dtype, size_t* meta_bytes, size_t* partial_out_bytes,
                               size_t* partial_lse_bytes) {
   if (int rc = check_plan(plan)) return rc;
-  if (kv_dtype != FCA_BF16 && kv_dtype != FCA_FP8_E4M3 && kv_dtype != FCA_F32)
+  if (kv_dtype != FCA_BF16 && kv_dtype != FCA_FP8_E4M3 && kv_dtype != FCA_FP8_E4M3_BLOCK && kv_dtype != FCA_F32)
     return fail(FCA_ERR_UNSUPPORTED, "kv_dtype %d is not supported (bf16, fp8 e4m3 or fp32)", kv_dtype);
   const fca::MetaLayout L = fca::make_layout(*plan);
   // one row per (partial slot, query head), then 32 rows per pair of waves that may share an item
@@ -427,6 +437,69 @@ int fca_gather_kv(void* key_dev, void* value_dev, int64_t token_stride, int64_t 
   return cache_rows(true, key_dev, value_dev, token_stride, head_stride, num_tokens, num_kv_heads, head_dim, slot_mapping_dev,
                     const_cast<void*>(k_cache_dev), const_cast<void*>(v_cache_dev), kv_block_stride, kv_head_stride, kv_dtype,
                     k_scale_dev, v_scale_dev, stream);
+}
+
+static int cache_rows_block(bool gather, const void* key_dev, const void* value_dev, int64_t token_stride, int64_t head_stride,
+                            int32_t num_tokens, int32_t num_kv_heads, int32_t head_dim, const int64_t* slot_mapping_dev,
+                            void* k_cache_dev, void* v_cache_dev, int64_t kv_block_stride, int64_t kv_head_stride,
+                            int64_t num_blocks, float* block_scales_dev, void* stream) {
+  if (num_tokens < 0 || num_kv_heads < 1) return fail(FCA_ERR_INVALID_ARG, "num_tokens must be >= 0 and num_kv_heads >= 1");
+  if (head_dim != 64 && head_dim != 128 && head_dim != 256)
+    return fail(FCA_ERR_UNSUPPORTED, "head_dim %d is not supported (64, 128 or 256)", head_dim);
+  if (num_blocks < 0 || num_blocks > 0x7fffffffLL)
+    return fail(FCA_ERR_INVALID_ARG, "num_blocks %lld must lie in [0, 2^31)", (long long)num_blocks);
+  if (num_tokens == 0) return FCA_OK;
+  if (!key_dev || !value_dev || !slot_mapping_dev || !k_cache_dev || !v_cache_dev || !block_scales_dev)
+    return fail(FCA_ERR_INVALID_ARG, "key, value, slot_mapping, the cache planes and block_scales must be non-NULL");
+  if ((reinterpret_cast<uintptr_t>(key_dev) & 15) || (reinterpret_cast<uintptr_t>(value_dev) & 15) || token_stride % 8 ||
+      head_stride % 8)
+    return fail(FCA_ERR_INVALID_ARG, "key and value must be 16-byte aligned with strides that are multiples of 8 elements");
+  if ((reinterpret_cast<uintptr_t>(k_cache_dev) & 15) || (reinterpret_cast<uintptr_t>(v_cache_dev) & 15) || kv_block_stride % 16 ||
+      kv_head_stride % 16 || kv_head_stride < (int64_t)FCA_BLOCK_SIZE * head_dim)
+    return fail(FCA_ERR_INVALID_ARG, "KV cache planes must be 16-byte aligned with 16-byte-multiple strides of at least one tile");
+  if (reinterpret_cast<uintptr_t>(block_scales_dev) & 7) return fail(FCA_ERR_INVALID_ARG, "block_scales must be 8-byte aligned");
+  fca::BlockCacheParams a{};
+  a.token_stride = token_stride;
+  a.head_stride = head_stride;
+  a.k_cache = k_cache_dev;
+  a.v_cache = v_cache_dev;
+  a.cache_block_stride = kv_block_stride;
+  a.cache_head_stride = kv_head_stride;
+  a.scales = block_scales_dev;
+  a.num_blocks = num_blocks;
+  a.num_kv_heads = num_kv_heads;
+  a.head_dim = head_dim;
+  // (the writer's workgroups look at every slot of a launch; the reader's grid stays within 31 bits)
+  const int32_t most = gather ? 1 << 24 : fca::kAppendTokens;
+  for (int32_t t0 = 0; t0 < num_tokens; t0 += most) {
+    a.num_tokens = num_tokens - t0 < most ? num_tokens - t0 : most;
+    a.key = static_cast<const char*>(key_dev) + 2 * (int64_t)t0 * token_stride;
+    a.value = static_cast<const char*>(value_dev) + 2 * (int64_t)t0 * token_stride;
+    a.slot_mapping = slot_mapping_dev + t0;
+    hipError_t e = gather ? fca::launch_gather_block(a, static_cast<hipStream_t>(stream))
+                          : fca::launch_append_block(a, static_cast<hipStream_t>(stream));
+    if (e != hipSuccess) return hip_fail(e, gather ? "block-scaled cache gather launch" : "block-scaled cache append launch");
+    if (num_tokens - t0 <= most) break;  // (t0 + most may pass 32 bits)
+  }
+  return FCA_OK;
+}
+
+int fca_append_kv_block_scaled(const void* key_dev, const void* value_dev, int64_t token_stride, int64_t head_stride,
+                               int32_t num_tokens, int32_t num_kv_heads, int32_t head_dim, const int64_t* slot_mapping_dev,
+                               void* k_cache_dev, void* v_cache_dev, int64_t kv_block_stride, int64_t kv_head_stride,
+                               int64_t num_blocks, float* block_scales_dev, void* stream) {
+  return cache_rows_block(false, key_dev, value_dev, token_stride, head_stride, num_tokens, num_kv_heads, head_dim,
+                          slot_mapping_dev, k_cache_dev, v_cache_dev, kv_block_stride, kv_head_stride, num_blocks,
+                          block_scales_dev, stream);
+}
+
+int fca_gather_kv_block_scaled(void* key_dev, void* value_dev, int64_t token_stride, int64_t head_stride, int32_t num_tokens,
+                               int32_t num_kv_heads, int32_t head_dim, const int64_t* slot_mapping_dev, const void* k_cache_dev,
+                               const void* v_cache_dev, int64_t kv_block_stride, int64_t kv_head_stride, int64_t num_blocks,
+                               const float* block_scales_dev, void* stream) {
+  return cache_rows_block(true, key_dev, value_dev, token_stride, head_stride, num_tokens, num_kv_heads, head_dim,
+                          slot_mapping_dev, const_cast<void*>(k_cache_dev), const_cast<void*>(v_cache_dev), kv_block_stride,
+                          kv_head_stride, num_blocks, const_cast<float*>(block_scales_dev), stream);
 }
 
 int fca_time_next_attention(void* start_event, void* stop_event) {

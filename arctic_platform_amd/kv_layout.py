@@ -13,6 +13,10 @@ operands with one contiguous 16-byte read per lane and no shuffle:
 This is the split layout the vLLM ROCm paged-attention path uses for its cache, so a
 stock ROCm backend can serve the prefill side of the same cache.
 
+A float8_e4m3fn cache comes in two forms: with one scale per KV head, given by the caller, or
+block-scaled: a fp32 table ``[num_blocks, num_kv_heads, 2]`` beside the cache holds one scale per
+block, KV head and plane (K's, V's), which the cache writer takes from the data.
+
 The attention-backend hook ``get_kv_cache_shape`` of the engine that the platform starts
 (``arctic_platform/common/ray_server.py:395-404``) is where this shape is announced.
 """
@@ -33,6 +37,12 @@ def kv_cache_shape(num_blocks: int, block_size: int, num_kv_heads: int, head_dim
     if block_size != BLOCK_SIZE:
         raise ValueError(f"forest cascade attention supports block_size={BLOCK_SIZE} only, got {block_size}")
     return (2, num_blocks, num_kv_heads, block_size * head_dim)
+
+
+def block_scales_shape(num_blocks: int, num_kv_heads: int):
+    """Shape of the fp32 scale table of a block-scaled cache.  The table needs no initial values (a
+    block's scales are written with its first token); zeros are a good choice."""
+    return (num_blocks, num_kv_heads, 2)
 
 
 def pack_blocks(k: torch.Tensor, v: torch.Tensor, dtype: torch.dtype | None = None) -> torch.Tensor:
@@ -67,3 +77,33 @@ def convert_cache(cache: torch.Tensor, head_dim: int, dtype: torch.dtype) -> tor
     """Re-pack a cache for another element type (the slice width ``x`` depends on it)."""
     k, v = unpack_blocks(cache, head_dim)
     return pack_blocks(k.to(dtype), v.to(dtype), dtype)
+
+
+E4M3_MAX = 448.0
+SCALE_EXP_MIN, SCALE_EXP_MAX = -100, 120
+
+
+def block_scale_for(amax: torch.Tensor) -> torch.Tensor:
+    """The smallest power of two s with ``amax <= 448 s``, kept within [2**-100, 2**120] (fp32)."""
+    m, e = torch.frexp(amax.float())  # amax = m * 2**e with m in [0.5, 1); 448 = 0.875 * 2**9
+    e = torch.where(m > 0.875, e + 1, e) - 9
+    e = torch.where(amax > 0, e, torch.full_like(e, SCALE_EXP_MIN)).clamp(SCALE_EXP_MIN, SCALE_EXP_MAX)
+    return ((e.to(torch.int32) + 127) << 23).view(torch.float32)
+
+
+def quantize_blocks(k: torch.Tensor, v: torch.Tensor):
+    """Token-major blocks ``[num_blocks, 16, num_kv_heads, head_dim]`` -> ``(cache, block_scales)`` as
+    ``append_kv(..., block_scales=)`` leaves them when whole blocks are written."""
+    codes, scales = [], []
+    for x in (k.float(), v.float()):
+        finite = torch.where(torch.isfinite(x), x.abs(), torch.zeros_like(x))
+        s = block_scale_for(finite.amax(dim=(1, 3)))
+        codes.append((x / s[:, None, :, None]).clamp(-E4M3_MAX, E4M3_MAX).to(torch.float8_e4m3fn))
+        scales.append(s)
+    return pack_blocks(*codes), torch.stack(scales, dim=-1).contiguous()
+
+
+def dequantize_blocks(cache: torch.Tensor, block_scales: torch.Tensor, head_dim: int):
+    """The way back: fp32 token-major ``(k, v)`` blocks of a block-scaled cache."""
+    k, v = unpack_blocks(cache, head_dim)
+    return k.float() * block_scales[:, None, :, 0:1], v.float() * block_scales[:, None, :, 1:2]

@@ -19,11 +19,12 @@ import ctypes
 import torch
 
 from . import _lib
+from .cache import check_block_scales, on_device
 from .forest import ForestMetadata, _stream_ptr
 from .kv_layout import BLOCK_SIZE
 
 
-def _tensors(q, kv_cache, meta: ForestMetadata, scale, k_scale, v_scale, f32_ok=False) -> _lib.FcaTensors:
+def _tensors(q, kv_cache, meta: ForestMetadata, scale, k_scale, v_scale, f32_ok=False, block_scales=None) -> _lib.FcaTensors:
     plan = meta.plan
     if q.dtype == torch.float32 or kv_cache.dtype == torch.float32:
         # the all-fp32 path: fp32 queries on an fp32 cache, fp32 partial rows
@@ -55,6 +56,13 @@ def _tensors(q, kv_cache, meta: ForestMetadata, scale, k_scale, v_scale, f32_ok=
     for name, sc in (("k_scale", k_scale), ("v_scale", v_scale)):
         if sc is not None and (sc.dtype != torch.float32 or sc.shape != (plan.num_kv_heads,) or not sc.is_contiguous()):
             raise ValueError(f"{name} must be a contiguous fp32 tensor of shape [{plan.num_kv_heads}]")
+    if block_scales is not None:
+        check_block_scales(block_scales, kv_cache, k_scale, v_scale)
+        if not (scale > 0):
+            raise ValueError(f"scale must be positive, got {scale}")
+        if not q.device == kv_cache.device == meta.meta.device:
+            raise ValueError("q, the cache and the metadata must be on one device")
+        kv_dtype, k_scale = _lib.FCA_FP8_E4M3_BLOCK, block_scales
     esz = kv_cache.element_size()
     return _lib.FcaTensors(
         q.data_ptr(),
@@ -103,88 +111,98 @@ def _out_args(q, meta, out, out_dtype):
 
 
 def forest_cascade_decode(
-    q, kv_cache, meta: ForestMetadata, scale, k_scale=None, v_scale=None, out=None, return_lse=True, out_dtype=None
+    q, kv_cache, meta: ForestMetadata, scale, k_scale=None, v_scale=None, out=None, return_lse=True, out_dtype=None,
+    block_scales=None,
 ):
     """One layer's decode attention.  Returns ``out`` or ``(out, lse)``.  ``q`` and ``kv_cache``
     in float32 take the all-fp32 path (fp32 products and partial rows; ``out`` then defaults to
-    float32): the metadata must have been built with ``partial_dtype=torch.float32``."""
+    float32): the metadata must have been built with ``partial_dtype=torch.float32``.
+    ``block_scales`` (fp32 ``[num_blocks, Hkv, 2]``) makes an fp8 cache a block-scaled one
+    (``append_kv``): every block of every KV head has a K and a V scale of its own."""
     lib = _lib.load_library()
-    t = _tensors(q, kv_cache, meta, scale, k_scale, v_scale, f32_ok=True)
+    t = _tensors(q, kv_cache, meta, scale, k_scale, v_scale, f32_ok=True, block_scales=block_scales)
     _check_partials(meta, t)
     out, code = _out_args(q, meta, out, out_dtype or (torch.float32 if t.kv_dtype == _lib.FCA_F32 else None))
     lse = torch.empty(meta.plan.num_seqs, meta.plan.num_q_heads, dtype=torch.float32, device=q.device) if return_lse else None
-    _lib.check(
-        lib.fca_decode_step(
-            ctypes.byref(meta.plan),
-            ctypes.byref(t),
-            meta.meta.data_ptr(),
-            meta.partial_out.data_ptr(),
-            meta.partial_lse.data_ptr(),
-            out.data_ptr(),
-            out.stride(0),
-            out.stride(1),
-            code,
-            lse.data_ptr() if lse is not None else None,
-            _stream_ptr(q.device),
+    with on_device(q.device):
+        _lib.check(
+            lib.fca_decode_step(
+                ctypes.byref(meta.plan),
+                ctypes.byref(t),
+                meta.meta.data_ptr(),
+                meta.partial_out.data_ptr(),
+                meta.partial_lse.data_ptr(),
+                out.data_ptr(),
+                out.stride(0),
+                out.stride(1),
+                code,
+                lse.data_ptr() if lse is not None else None,
+                _stream_ptr(q.device),
+            )
         )
-    )
     return (out, lse) if return_lse else out
 
 
-def forest_cascade_decode_static(q, kv_cache, meta: ForestMetadata, scale, k_scale=None, v_scale=None, *, out, lse=None):
+def forest_cascade_decode_static(
+    q, kv_cache, meta: ForestMetadata, scale, k_scale=None, v_scale=None, *, out, lse=None, block_scales=None
+):
     """``forest_cascade_decode`` on the library's own partial buffers
     (``fca_decode_step_static``): nothing is allocated, so ``out`` (and ``lse`` if wanted)
     must be passed in, and ``meta.partial_out`` / ``meta.partial_lse`` are not touched.
     Plans whose partial rows exceed ``_lib.FCA_STATIC_SCRATCH_BYTES`` raise.  All calls on
     one GPU share the buffers: keep them in stream order."""
     lib = _lib.load_library()
-    t = _tensors(q, kv_cache, meta, scale, k_scale, v_scale, f32_ok=True)
+    t = _tensors(q, kv_cache, meta, scale, k_scale, v_scale, f32_ok=True, block_scales=block_scales)
     out, code = _out_args(q, meta, out, None)
     if lse is not None and (lse.dtype != torch.float32 or lse.shape != (meta.plan.num_seqs, meta.plan.num_q_heads) or not lse.is_contiguous()):
         raise ValueError("lse must be a contiguous fp32 tensor [num_seqs, num_q_heads]")
-    _lib.check(
-        lib.fca_decode_step_static(
-            ctypes.byref(meta.plan), ctypes.byref(t), meta.meta.data_ptr(), out.data_ptr(), out.stride(0), out.stride(1),
-            code, lse.data_ptr() if lse is not None else None, _stream_ptr(q.device),
+    with on_device(q.device):
+        _lib.check(
+            lib.fca_decode_step_static(
+                ctypes.byref(meta.plan), ctypes.byref(t), meta.meta.data_ptr(), out.data_ptr(), out.stride(0), out.stride(1),
+                code, lse.data_ptr() if lse is not None else None, _stream_ptr(q.device),
+            )
         )
-    )
     return out if lse is None else (out, lse)
 
 
-def prefix_pass(q, kv_cache, meta: ForestMetadata, scale, k_scale=None, v_scale=None):
+def prefix_pass(q, kv_cache, meta: ForestMetadata, scale, k_scale=None, v_scale=None, block_scales=None):
     """Shared-node work items only; fills their slots of the partial buffers."""
     lib = _lib.load_library()
-    t = _tensors(q, kv_cache, meta, scale, k_scale, v_scale)
-    _lib.check(
-        lib.fca_prefix_pass(
-            ctypes.byref(meta.plan), ctypes.byref(t), meta.meta.data_ptr(), meta.partial_out.data_ptr(),
-            meta.partial_lse.data_ptr(), _stream_ptr(q.device),
+    t = _tensors(q, kv_cache, meta, scale, k_scale, v_scale, block_scales=block_scales)
+    with on_device(q.device):
+        _lib.check(
+            lib.fca_prefix_pass(
+                ctypes.byref(meta.plan), ctypes.byref(t), meta.meta.data_ptr(), meta.partial_out.data_ptr(),
+                meta.partial_lse.data_ptr(), _stream_ptr(q.device),
+            )
         )
-    )
 
 
-def suffix_pass(q, kv_cache, meta: ForestMetadata, scale, k_scale=None, v_scale=None):
+def suffix_pass(q, kv_cache, meta: ForestMetadata, scale, k_scale=None, v_scale=None, block_scales=None):
     """Private-leaf work items only; fills their slots of the partial buffers."""
     lib = _lib.load_library()
-    t = _tensors(q, kv_cache, meta, scale, k_scale, v_scale)
-    _lib.check(
-        lib.fca_suffix_pass(
-            ctypes.byref(meta.plan), ctypes.byref(t), meta.meta.data_ptr(), meta.partial_out.data_ptr(),
-            meta.partial_lse.data_ptr(), _stream_ptr(q.device),
+    t = _tensors(q, kv_cache, meta, scale, k_scale, v_scale, block_scales=block_scales)
+    with on_device(q.device):
+        _lib.check(
+            lib.fca_suffix_pass(
+                ctypes.byref(meta.plan), ctypes.byref(t), meta.meta.data_ptr(), meta.partial_out.data_ptr(),
+                meta.partial_lse.data_ptr(), _stream_ptr(q.device),
+            )
         )
-    )
 
 
-def forest_pass(q, kv_cache, meta: ForestMetadata, scale, k_scale=None, v_scale=None):
+def forest_pass(q, kv_cache, meta: ForestMetadata, scale, k_scale=None, v_scale=None, block_scales=None):
     """Shared and private work items in one launch; fills every live partial slot."""
     lib = _lib.load_library()
-    t = _tensors(q, kv_cache, meta, scale, k_scale, v_scale)
-    _lib.check(
-        lib.fca_forest_pass(
-            ctypes.byref(meta.plan), ctypes.byref(t), meta.meta.data_ptr(), meta.partial_out.data_ptr(),
-            meta.partial_lse.data_ptr(), _stream_ptr(q.device),
+    t = _tensors(q, kv_cache, meta, scale, k_scale, v_scale, block_scales=block_scales)
+    with on_device(q.device):
+        _lib.check(
+            lib.fca_forest_pass(
+                ctypes.byref(meta.plan), ctypes.byref(t), meta.meta.data_ptr(), meta.partial_out.data_ptr(),
+                meta.partial_lse.data_ptr(), _stream_ptr(q.device),
+            )
         )
-    )
 
 
 def merge_partials(meta: ForestMetadata, q_like, out=None, return_lse=True, out_dtype=None):

@@ -59,7 +59,13 @@ typedef enum fca_status {
 typedef enum fca_dtype {
   FCA_BF16 = 0,     /* q, out, KV cache */
   FCA_FP8_E4M3 = 1, /* KV cache only (OCP e4m3fn) */
-  FCA_F32 = 2       /* out; as kv_dtype: q and the KV cache are fp32 */
+  FCA_F32 = 2,      /* out; as kv_dtype: q and the KV cache are fp32 */
+  /* KV cache only: e4m3 codes in the layout of FCA_FP8_E4M3, with one positive fp32 scale per
+   * (block, KV head) and plane in a table [num_blocks, Hkv, 2] (K's, V's) next to the cache; a
+   * code c stands for c * scale.  Filled by fca_append_kv_block_scaled, read back by
+   * fca_gather_kv_block_scaled; the attention calls take the table in
+   * fca_tensors.k_scale_dev, with v_scale_dev NULL.  Partial rows as for FCA_FP8_E4M3. */
+  FCA_FP8_E4M3_BLOCK = 3
 } fca_dtype;
 
 /* Shape of one decode batch and the tiling the metadata is built for. */
@@ -84,14 +90,15 @@ typedef struct fca_tensors {
   const void* v_cache_dev;     /* V plane: [num_blocks, Hkv, D, 16] */
   int64_t kv_block_stride;     /* elements between blocks of one plane */
   int64_t kv_head_stride;      /* elements between KV heads of one block */
-  int32_t kv_dtype;            /* FCA_BF16, FCA_FP8_E4M3, or FCA_F32 (then q is fp32 as well) */
+  int32_t kv_dtype;            /* FCA_BF16, FCA_FP8_E4M3, FCA_FP8_E4M3_BLOCK, or FCA_F32 (then q is fp32 as well) */
   int32_t kv_reread;           /* 0: a launch reads every KV block about once (decode), loads bypass
                                   the caches; non-zero: blocks are read again and again (query runs
                                   built with fca_build_metadata_rows), loads stay cacheable */
   const int32_t* block_table_dev; /* [S, max_blocks] physical block ids ([table_rows, max_blocks]
                                   for metadata built with fca_build_metadata_rows) */
   int64_t block_table_stride;
-  const float* k_scale_dev;    /* [Hkv] dequant scales for fp8 caches, or NULL (= 1) */
+  const float* k_scale_dev;    /* [Hkv] dequant scales for fp8 caches, or NULL (= 1); FCA_FP8_E4M3_BLOCK:
+                                  the scale table [num_blocks, Hkv, 2], 8-byte aligned */
   const float* v_scale_dev;
   float softmax_scale;         /* usually head_dim ** -0.5 */
   int32_t reproducible;        /* non-zero: no work item is attended by two waves together, so where an
@@ -292,6 +299,38 @@ int fca_gather_kv(void* key_dev, void* value_dev, int64_t token_stride, int64_t 
                   int32_t num_kv_heads, int32_t head_dim, const int64_t* slot_mapping_dev, const void* k_cache_dev,
                   const void* v_cache_dev, int64_t kv_block_stride, int64_t kv_head_stride, int32_t kv_dtype,
                   const float* k_scale_dev, const float* v_scale_dev, void* stream);
+
+/* ---- the block-scaled 8-bit cache (kv_dtype FCA_FP8_E4M3_BLOCK) ---------------------------
+ * Writing with the scales taken from the data, where fca_append_kv needs them beforehand.  For
+ * every (block, KV head, plane) that tokens of the call fall into, with a = the largest finite
+ * magnitude among those tokens:
+ *   need  = the smallest power of two s with a <= 448 s, kept within [2^-100, 2^120]
+ *   old   = nothing if one of the tokens has offset 0 of the block, else the block's scale
+ *           (nothing too if that is no positive finite number; raised to a power of two if it
+ *           is none)
+ *   scale = max(old, need), written to the table
+ *   codes of the call's tokens = clamp(x / scale, +-448) to e4m3, nearest, ties to even
+ *           (infinities saturate, NaN is stored as NaN and does not touch the scale)
+ *   where scale > old, codes c of the block's other tokens become e4m3(c * old / scale).
+ * So offset 0 begins a block: what the block held before is forgotten, and its scale with it
+ * (blocks are used again without being cleared); the tokens behind it have to be written in that
+ * call or after it.  Writing a token again is allowed; the scale of a begun block never falls.
+ * Tokens of one call may come in any order; of two with the same slot the later one is stored.
+ * A negative slot is padding; a slot of a block beyond num_blocks is skipped like padding.  Calls
+ * of more than 32768 tokens have the effect of successive calls of 32768.
+ * slot_mapping, key, value, strides: as for fca_append_kv (bf16 rows).  block_scales:
+ * [num_blocks, Hkv, 2] fp32, contiguous, 8-byte aligned.  Calls that touch one block must be in
+ * stream order, and so must reads of it.  One launch per 32768 tokens, no workspace. */
+int fca_append_kv_block_scaled(const void* key_dev, const void* value_dev, int64_t token_stride, int64_t head_stride,
+                               int32_t num_tokens, int32_t num_kv_heads, int32_t head_dim, const int64_t* slot_mapping_dev,
+                               void* k_cache_dev, void* v_cache_dev, int64_t kv_block_stride, int64_t kv_head_stride,
+                               int64_t num_blocks, float* block_scales_dev, void* stream);
+/* The way back: key[t], value[t] = code * scale of slot_mapping[t] as bf16 rows (zeros for a
+ * negative slot or one beyond num_blocks). */
+int fca_gather_kv_block_scaled(void* key_dev, void* value_dev, int64_t token_stride, int64_t head_stride, int32_t num_tokens,
+                               int32_t num_kv_heads, int32_t head_dim, const int64_t* slot_mapping_dev, const void* k_cache_dev,
+                               const void* v_cache_dev, int64_t kv_block_stride, int64_t kv_head_stride, int64_t num_blocks,
+                               const float* block_scales_dev, void* stream);
 
 /* ---- split attention of the trainer (forward and backward) ---------------------------
  * Attention over a deduplicated, unpadded training batch: q [T, Hq, D], k and v
