@@ -28,6 +28,12 @@ __all__ = [
 def __getattr__(name):
     # operators need the HIP library; resolve them lazily so the flag parser and layout
     # helpers stay importable in a process that only builds or inspects
+    value = _resolve(name)
+    globals()[name] = value  # (found here from now on)
+    return value
+
+
+def _resolve(name):
     if name in ("build_forest_metadata", "ForestMetadata"):
         from . import forest
 

@@ -22,14 +22,17 @@ from .kv_layout import BLOCK_SIZE, block_scales_shape
 
 def on_device(device):
     """A launch goes to the current device: makes ``device`` that for a call on another one's tensors."""
-    if device.type != "cuda" or device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
+    if device.type != "cuda" or device.index == torch._C._cuda_getDevice():
+        return _CURRENT
     return torch.cuda.device(device)
+
+
+_CURRENT = contextlib.nullcontext()
 
 
 def check_block_scales(block_scales, kv_cache, k_scale, v_scale) -> None:
     """The scale table of a block-scaled cache (``kv_layout.block_scales_shape``) against its cache."""
-    if kv_cache.dtype != torch.float8_e4m3fn:
+    if kv_cache.dtype != torch.float8_e4m3fn or kv_cache.dim() != 4:
         raise TypeError(f"block_scales belong to a float8_e4m3fn cache, got {kv_cache.dtype}")
     if k_scale is not None or v_scale is not None:
         raise ValueError("a cache has either block_scales or per-head k_scale / v_scale")
@@ -67,6 +70,9 @@ def append_kv(key, value, kv_cache, slot_mapping, k_scale=None, v_scale=None, bl
 
 
 def _cache_rows(gather, key, value, kv_cache, slot_mapping, k_scale, v_scale, block_scales=None) -> None:
+    if block_scales is not None:
+        check_block_scales(block_scales, kv_cache, k_scale, v_scale)
+        return _block_scaled_rows(gather, key, value, kv_cache, slot_mapping, block_scales)
     f32 = kv_cache.dtype == torch.float32
     rows_dtype = torch.float32 if f32 else torch.bfloat16
     if key.dtype != rows_dtype or value.dtype != rows_dtype or key.shape != value.shape or key.dim() != 3:
@@ -98,19 +104,6 @@ def _cache_rows(gather, key, value, kv_cache, slot_mapping, k_scale, v_scale, bl
         if sc is not None and (sc.dtype != torch.float32 or sc.shape != (hkv,) or not sc.is_contiguous()):
             raise ValueError(f"{name} must be a contiguous fp32 tensor of shape [{hkv}]")
     lib = _lib.load_library()
-    if block_scales is not None:
-        check_block_scales(block_scales, kv_cache, k_scale, v_scale)
-        if not key.device == value.device == kv_cache.device == slot_mapping.device:
-            raise ValueError("key, value, slot_mapping and the cache must be on one device")
-        with on_device(kv_cache.device):
-            _lib.check(
-                (lib.fca_gather_kv_block_scaled if gather else lib.fca_append_kv_block_scaled)(
-                    key.data_ptr(), value.data_ptr(), key.stride(0), key.stride(1), t, hkv, d, slot_mapping.data_ptr(),
-                    kv_cache.data_ptr(), kv_cache.data_ptr() + kv_cache.stride(0), kv_cache.stride(1), kv_cache.stride(2),
-                    kv_cache.shape[1], block_scales.data_ptr(), _stream_ptr(kv_cache.device),
-                )
-            )
-        return
     esz = kv_cache.element_size()
     _lib.check(
         (lib.fca_gather_kv if gather else lib.fca_append_kv)(
@@ -120,3 +113,35 @@ def _cache_rows(gather, key, value, kv_cache, slot_mapping, k_scale, v_scale, bl
             _stream_ptr(key.device),
         )
     )
+
+
+def _block_scaled_rows(gather, key, value, kv_cache, slot_mapping, block_scales) -> None:
+    if key.dtype != torch.bfloat16 or value.dtype != torch.bfloat16:
+        raise TypeError("key and value must be bfloat16 for a block-scaled cache")
+    shape, strides = key.shape, key.stride()
+    if len(shape) != 3 or value.shape != shape:
+        raise TypeError("key and value must be of the same shape [tokens, kv_heads, head_dim]")
+    if value.stride() != strides or strides[2] != 1:
+        raise ValueError("key and value must share strides and have a contiguous head_dim")
+    t, hkv, d = shape
+    if slot_mapping.dtype != torch.int64 or slot_mapping.shape != (t,) or not slot_mapping.is_contiguous():
+        raise ValueError("slot_mapping must be a contiguous int64 tensor of shape [tokens]")
+    cache_strides = kv_cache.stride()
+    if kv_cache.dim() != 4 or kv_cache.shape[0] != 2 or kv_cache.shape[2] != hkv or kv_cache.shape[3] != BLOCK_SIZE * d or cache_strides[3] != 1:
+        raise ValueError("kv_cache must be [2, num_blocks, num_kv_heads, 16 * head_dim] with contiguous tiles")
+    device = kv_cache.device
+    if not kv_cache.is_cuda:
+        raise RuntimeError("append_kv runs on the GPU only")
+    if not key.device == value.device == slot_mapping.device == device:
+        raise ValueError("key, value, slot_mapping and the cache must be on one device")
+    lib = _lib.load_library()
+    entry = lib.fca_gather_kv_block_scaled if gather else lib.fca_append_kv_block_scaled
+    base = kv_cache.data_ptr()
+    with on_device(device):
+        _lib.check(
+            entry(
+                key.data_ptr(), value.data_ptr(), strides[0], strides[1], t, hkv, d, slot_mapping.data_ptr(), base,
+                base + cache_strides[0], cache_strides[1], cache_strides[2], kv_cache.shape[1], block_scales.data_ptr(),
+                _stream_ptr(device),
+            )
+        )

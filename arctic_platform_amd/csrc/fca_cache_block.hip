@@ -7,7 +7,7 @@
 //   scale' = max(old, need)
 //   codes of the call's tokens = e4m3(x / scale'), nearest, ties to even, saturating; NaN stays NaN
 //   where scale' > old, the codes of the other tokens become e4m3(c * old / scale')
-// All tokens of a call that fall into one block are handled by the same workgroup, so the scale is
+// All tokens of a call that fall into one block are handled by the same workgroups, so the scale is
 // a maximum over all of them and nothing depends on the order of workgroups: no atomics on global
 // memory, no workspace, one launch.  Of two tokens with one slot the later one is written.
 //
@@ -21,9 +21,11 @@
 
 namespace fca {
 
-typedef int i32x4_t __attribute__((ext_vector_type(4)));
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
 
 __device__ inline float bf16_float(unsigned short x) { return __uint_as_float((unsigned)x << 16); }
+__device__ inline float bf16_low(unsigned w) { return __uint_as_float(w << 16); }
+__device__ inline float bf16_high(unsigned w) { return __uint_as_float(w & 0xffff0000u); }
 
 __device__ inline unsigned e4m3_code(float x) {
   // saturate (clamp, then round to nearest even); NaN is stored as the canonical 0x7f
@@ -31,29 +33,63 @@ __device__ inline unsigned e4m3_code(float x) {
   x = fminf(fmaxf(x, -kE4m3Max), kE4m3Max);
   return (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(x, 0.f, 0, false) & 0xff;
 }
-// One byte of a dword of codes, scaled and rounded again.
-__device__ inline unsigned rescaled_code(unsigned codes, int byte, float ratio) {
-  return e4m3_code(__builtin_amdgcn_cvt_f32_fp8((int)(codes >> (8 * byte)), 0) * ratio);
+__device__ inline unsigned e4m3_codes(float a, float b, float c, float d) {
+  return e4m3_code(a) | e4m3_code(b) << 8 | e4m3_code(c) << 16 | e4m3_code(d) << 24;
+}
+// The same for numbers that are known to lie within +-448.
+__device__ inline unsigned e4m3_codes_of_small(float a, float b, float c, float d) {
+  return (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false), true);
+}
+// Four codes, scaled by at most 1 and rounded again (a code that is NaN may be among them).
+__device__ inline unsigned rescaled_codes(unsigned w, float ratio) {
+  return e4m3_codes(__builtin_amdgcn_cvt_f32_fp8((int)w, 0) * ratio, __builtin_amdgcn_cvt_f32_fp8((int)(w >> 8), 0) * ratio,
+                    __builtin_amdgcn_cvt_f32_fp8((int)(w >> 16), 0) * ratio, __builtin_amdgcn_cvt_f32_fp8((int)(w >> 24), 0) * ratio);
 }
 
-__device__ inline float finite_max(float m, unsigned short x) {
-  const unsigned short a = x & 0x7fff;
-  return a < 0x7f80 ? fmaxf(m, bf16_float(a)) : m;
+// Largest magnitudes of pairs of bf16 numbers, as bit patterns: magnitudes order like integers.
+__device__ inline u16x2 pair_max(u16x2 m, unsigned w) {
+  const u16x2 x = __builtin_bit_cast(u16x2, w & 0x7fff7fffu);
+  return u16x2{x[0] > m[0] ? x[0] : m[0], x[1] > m[1] ? x[1] : m[1]};
+}
+__device__ inline unsigned short finite_max(unsigned short m, unsigned w) {
+  const unsigned short lo = w & 0x7fff, hi = (w >> 16) & 0x7fff;
+  if (lo < 0x7f80 && lo > m) m = lo;
+  if (hi < 0x7f80 && hi > m) m = hi;
+  return m;
+}
+// The lane's largest finite magnitude in `n` dwords; `special`: an infinity or a NaN is among them.
+template <int N>
+__device__ inline unsigned short lane_max(const unsigned (&w)[N], bool& special) {
+  u16x2 pm = {0, 0};
+#pragma unroll
+  for (int i = 0; i < N; ++i) pm = pair_max(pm, w[i]);
+  unsigned short m = pm[0] > pm[1] ? pm[0] : pm[1];
+  special = m >= 0x7f80;
+  if (special) {
+    m = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) m = finite_max(m, w[i]);
+  }
+  return m;
 }
 
 // The scale of one (block, head, plane): what it was, what it becomes.
 struct ScaleStep {
-  float inv;    // 1 / new scale
-  float ratio;  // old / new, for the codes that stay
-  bool grown;   // codes that stay have to be rescaled
+  float inv;     // 1 / new scale
+  float ratio;   // old / new, for the codes that stay
+  bool grown;    // codes that stay have to be rescaled
+  bool special;  // infinities or NaNs among the tile's new values
 };
-__device__ inline ScaleStep step_scale(float* at, float amax, bool begins, int lane) {
-  const float was = *at;  // (every lane has it before the reduction, lane 0 writes behind it)
+__device__ inline ScaleStep step_scale(float* at, float was, unsigned lane_amax, bool lane_special, bool begins, int lane) {
+  unsigned amax = lane_amax;  // (bit patterns of bf16 magnitudes: their order is that of the numbers)
 #pragma unroll
-  for (int off = 32; off > 0; off >>= 1) amax = fmaxf(amax, __shfl_xor(amax, off));
+  for (int off = 32; off > 0; off >>= 1) {
+    const unsigned o = __shfl_xor(amax, off);
+    amax = o > amax ? o : amax;
+  }
   // (a scale that is no positive finite number, of a block nothing has begun, counts for nothing)
   const bool has_old = !begins && was > 0.f && was < INFINITY;
-  int e = scale_exp_for(amax);
+  int e = scale_exp_for(bf16_float((unsigned short)amax));
   if (has_old) {
     const int eo = scale_exp_above(was);  // (a caller's own scale that is no power of two is raised to one)
     e = e > eo ? e : eo;
@@ -63,125 +99,195 @@ __device__ inline ScaleStep step_scale(float* at, float amax, bool begins, int l
   s.inv = __uint_as_float((unsigned)(254 - e) << 23);
   s.ratio = was * s.inv;
   s.grown = has_old && scale != was;
+  s.special = __ballot(lane_special) != 0;
   if (lane == 0 && scale != was) *at = scale;
   return s;
 }
 
+// `win`: the call's token at every offset of the block, -1 = none.
 template <int D>
 __device__ inline void append_k_tile(const BlockCacheParams& p, const int* win, int64_t blk, int h, int lane) {
   constexpr int U = D / 64;  // 16-byte units of the tile per lane
   const int tok = lane & 15;
   const int t = win[tok];
+  float* at = p.scales + (blk * p.num_kv_heads + h) * 2;
+  const float was = *at;  // (every lane has it before the reduction, lane 0 writes behind it)
   char* tile = static_cast<char*>(p.k_cache) + blk * p.cache_block_stride + h * p.cache_head_stride;
   const unsigned short* row = static_cast<const unsigned short*>(p.key) + (int64_t)t * p.token_stride + (int64_t)h * p.head_stride;
-  union {
-    int4 raw[2];
-    unsigned short x[16];
-  } in[U];
+  unsigned in[U * 8];
   union Codes {
     int4 raw;
     unsigned w[4];
   } out[U];
-  float amax = 0.f;
+#pragma unroll
+  for (int i = 0; i < U; ++i) {
+    const int c = (lane >> 4) + 4 * i;
+    int4 x0 = make_int4(0, 0, 0, 0), x1 = x0;
+    if (t >= 0) {
+      x0 = *reinterpret_cast<const int4*>(row + 16 * c);
+      x1 = *reinterpret_cast<const int4*>(row + 16 * c + 8);
+    } else {
+      out[i].raw = *reinterpret_cast<const int4*>(tile + (c * kBlock + tok) * 16);
+    }
+    in[8 * i] = x0.x, in[8 * i + 1] = x0.y, in[8 * i + 2] = x0.z, in[8 * i + 3] = x0.w;
+    in[8 * i + 4] = x1.x, in[8 * i + 5] = x1.y, in[8 * i + 6] = x1.z, in[8 * i + 7] = x1.w;
+  }
+  bool special;
+  const unsigned amax = lane_max(in, special);
+  const ScaleStep s = step_scale(at, was, amax, special, win[0] >= 0, lane);
+  if (t < 0 && !s.grown) return;
 #pragma unroll
   for (int i = 0; i < U; ++i) {
     const int c = (lane >> 4) + 4 * i;
     if (t >= 0) {
-      in[i].raw[0] = *reinterpret_cast<const int4*>(row + 16 * c);
-      in[i].raw[1] = *reinterpret_cast<const int4*>(row + 16 * c + 8);
 #pragma unroll
-      for (int e = 0; e < 16; ++e) amax = finite_max(amax, in[i].x[e]);
+      for (int d = 0; d < 4; ++d) {
+        const unsigned lo = in[8 * i + 2 * d], hi = in[8 * i + 2 * d + 1];
+        const float x0 = bf16_low(lo) * s.inv, x1 = bf16_high(lo) * s.inv, x2 = bf16_low(hi) * s.inv, x3 = bf16_high(hi) * s.inv;
+        out[i].w[d] = s.special ? e4m3_codes(x0, x1, x2, x3) : e4m3_codes_of_small(x0, x1, x2, x3);
+      }
     } else {
-      out[i].raw = *reinterpret_cast<const int4*>(tile + (c * kBlock + tok) * 16);
-    }
-  }
-  const ScaleStep s = step_scale(p.scales + (blk * p.num_kv_heads + h) * 2, amax, win[0] >= 0, lane);
 #pragma unroll
-  for (int i = 0; i < U; ++i) {
-    const int c = (lane >> 4) + 4 * i;
-    if (t < 0 && !s.grown) continue;
-#pragma unroll
-    for (int d = 0; d < 4; ++d) {
-      unsigned q = 0;
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        q |= (t >= 0 ? e4m3_code(bf16_float(in[i].x[4 * d + e]) * s.inv) : rescaled_code(out[i].w[d], e, s.ratio)) << (8 * e);
-      out[i].w[d] = q;
+      for (int d = 0; d < 4; ++d) out[i].w[d] = rescaled_codes(out[i].w[d], s.ratio);
     }
     *reinterpret_cast<int4*>(tile + (c * kBlock + tok) * 16) = out[i].raw;
+  }
+}
+
+// CH adjacent bf16 numbers (an element access of 2, 4 or 8 bytes) as dwords.
+template <int CH>
+__device__ inline void load_channels(const unsigned short* from, unsigned (&w)[(CH + 1) / 2]) {
+  if constexpr (CH == 1) {
+    w[0] = *from;
+  } else if constexpr (CH == 2) {
+    w[0] = *reinterpret_cast<const unsigned*>(from);
+  } else {
+    const uint2 x = *reinterpret_cast<const uint2*>(from);
+    w[0] = x.x, w[1] = x.y;
   }
 }
 
 template <int D>
 __device__ inline void append_v_tile(const BlockCacheParams& p, const int* win, int64_t blk, int h, int lane) {
   constexpr int CH = D / 64;  // adjacent channels per lane
+  constexpr int W = (CH + 1) / 2;
+  float* at = p.scales + (blk * p.num_kv_heads + h) * 2 + 1;
+  const float was = *at;
   char* tile = static_cast<char*>(p.v_cache) + blk * p.cache_block_stride + h * p.cache_head_stride + lane * CH * kBlock;
-  struct alignas(2 * CH) Piece {
-    unsigned short x[CH];
-  } in[kBlock];
+  const unsigned short* rows = static_cast<const unsigned short*>(p.value) + (int64_t)h * p.head_stride + lane * CH;
+  const int mine = win[lane & 15];
+  const unsigned live = (unsigned)(__ballot(mine >= 0) & 0xffff);
   union Codes {
     int4 raw;
     unsigned w[4];
-  } out[CH];
-  float amax = 0.f;
+  } old[CH];
+  if (live != 0xffff) {
 #pragma unroll
-  for (int ch = 0; ch < CH; ++ch) out[ch].raw = *reinterpret_cast<const int4*>(tile + ch * kBlock);
-  unsigned live = 0;
+    for (int ch = 0; ch < CH; ++ch) old[ch].raw = *reinterpret_cast<const int4*>(tile + ch * kBlock);
+  } else {
+#pragma unroll
+    for (int ch = 0; ch < CH; ++ch) old[ch].raw = make_int4(0, 0, 0, 0);
+  }
+  unsigned in[kBlock * W];
 #pragma unroll
   for (int k = 0; k < kBlock; ++k) {
-    const int t = __builtin_amdgcn_readfirstlane(win[k]);
-    if (t >= 0) {
-      live |= 1u << k;
-      in[k] = *reinterpret_cast<const Piece*>(static_cast<const unsigned short*>(p.value) + (int64_t)t * p.token_stride +
-                                              (int64_t)h * p.head_stride + lane * CH);
+    const int t = __builtin_amdgcn_readlane(mine, k);
+    unsigned w[W] = {};
+    if (t >= 0) load_channels<CH>(rows + (int64_t)t * p.token_stride, w);
 #pragma unroll
-      for (int ch = 0; ch < CH; ++ch) amax = finite_max(amax, in[k].x[ch]);
-    }
+    for (int i = 0; i < W; ++i) in[k * W + i] = w[i];
   }
-  const ScaleStep s = step_scale(p.scales + (blk * p.num_kv_heads + h) * 2 + 1, amax, win[0] >= 0, lane);
+  bool special;
+  const unsigned amax = lane_max(in, special);
+  const ScaleStep s = step_scale(at, was, amax, special, live & 1, lane);
 #pragma unroll
   for (int ch = 0; ch < CH; ++ch) {
 #pragma unroll
     for (int d = 0; d < 4; ++d) {
-      unsigned q = 0;
+      float x[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const int k = 4 * d + e;
-        const unsigned kept = s.grown ? rescaled_code(out[ch].w[d], e, s.ratio) : (out[ch].w[d] >> (8 * e)) & 0xff;
-        q |= ((live >> k) & 1 ? e4m3_code(bf16_float(in[k].x[ch]) * s.inv) : kept) << (8 * e);
+        const unsigned w = in[(4 * d + e) * W + ch / 2];
+        x[e] = (ch & 1 ? bf16_high(w) : bf16_low(w)) * s.inv;
       }
-      out[ch].w[d] = q;
+      const unsigned q = s.special ? e4m3_codes(x[0], x[1], x[2], x[3]) : e4m3_codes_of_small(x[0], x[1], x[2], x[3]);
+      // bytes of the call's tokens (the same in every lane)
+      const unsigned four = (live >> (4 * d)) & 15;
+      const unsigned fresh = ((four & 1) | (four & 2) << 7 | (four & 4) << 14 | (four & 8) << 21) * 0xffu;
+      const unsigned kept = s.grown ? rescaled_codes(old[ch].w[d], s.ratio) : old[ch].w[d];
+      old[ch].w[d] = (q & fresh) | (kept & ~fresh);
     }
-    *reinterpret_cast<int4*>(tile + ch * kBlock) = out[ch].raw;
+    *reinterpret_cast<int4*>(tile + ch * kBlock) = old[ch].raw;
   }
 }
 
-// One workgroup per token of the call; the first token of a block in the call owns the block.
+// A workgroup takes `window` successive tokens of the call and `heads` KV heads: it owns the blocks
+// whose first token of the call is among them.  Which of its blocks that holds for, and which later
+// tokens belong to them, it finds by looking at all slots of the call: they are few next to the rows
+// (8 bytes a token against 4 D Hkv), come out of the L2, and nothing has to be known about their order.
+constexpr int kMaxWindow = 64;
 template <int D>
-__global__ __launch_bounds__(256) void fca_append_block_kernel(BlockCacheParams p) {
-  __shared__ int win[kBlock];  // the call's token at every offset of the block, -1 = none
-  __shared__ int foreign;
-  const int t0 = blockIdx.x, tid = threadIdx.x;
-  const int64_t slot = p.slot_mapping[t0];
-  if (slot < 0 || slot >= p.num_blocks * kBlock) return;
-  const int64_t blk = slot / kBlock;
-  if (tid < kBlock) win[tid] = -1;
-  if (tid == 0) foreign = 0;
+__global__ __launch_bounds__(256) void fca_append_block_kernel(BlockCacheParams p, int window, int heads, int head_groups) {
+  __shared__ int cand[kMaxWindow];         // blocks of the window's tokens, each once
+  __shared__ int win[kMaxWindow][kBlock];  // the call's last token at every offset of theirs, -1 = none
+  __shared__ int foreign[kMaxWindow];      // the block has a token in front of the window
+  __shared__ int num_cand;
+  const int tid = threadIdx.x;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+  const int w = blockIdx.x / head_groups, h0 = (blockIdx.x - w * head_groups) * heads;
+  const int t0 = w * window;
+  const int64_t end = p.num_blocks * kBlock;
+  if (wave == 0) {
+    int blk = -1;
+    if (lane < window && t0 + lane < p.num_tokens) {
+      const int64_t slot = p.slot_mapping[t0 + lane];
+      if (slot >= 0 && slot < end) blk = (int)(slot / kBlock);
+    }
+    bool leads = blk >= 0;
+    for (int j = 0; j < window - 1; ++j) {
+      const int other = __builtin_amdgcn_readlane(blk, j);
+      if (j < lane && other == blk) leads = false;
+    }
+    const unsigned long long all = __ballot(leads);
+    if (leads) cand[__popcll(all & ((1ull << lane) - 1))] = blk;
+    if (lane == 0) num_cand = __popcll(all);
+  }
+  for (int j = tid; j < window * kBlock; j += 256) (&win[0][0])[j] = -1;
+  if (tid < kMaxWindow) foreign[tid] = 0;
   __syncthreads();
-  for (int t = tid; t < p.num_tokens; t += 256) {
-    const int64_t s = p.slot_mapping[t];
-    if (s < 0 || s / kBlock != blk) continue;
-    if (t < t0) foreign = 1;
-    atomicMax(&win[s % kBlock], t);
+  const int n = num_cand;
+  if (n == 0) return;
+  // (four slots per thread and trip: their loads are in flight together)
+  for (int base = 0; base < p.num_tokens; base += 1024) {
+    int blk[4], off[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int t = base + 256 * k + tid;
+      int64_t slot = -1;
+      if (t < p.num_tokens) slot = p.slot_mapping[t];
+      blk[k] = slot >= 0 && slot < end ? (int)(slot / kBlock) : -1;
+      off[k] = (int)(slot & (kBlock - 1));
+    }
+    for (int c = 0; c < n; ++c) {
+      const int mine = cand[c];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if (blk[k] != mine) continue;
+        const int t = base + 256 * k + tid;
+        if (t < t0) foreign[c] = 1;
+        else atomicMax(&win[c][off[k]], t);
+      }
+    }
   }
   __syncthreads();
-  if (foreign) return;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
-  for (int j = wave; j < 2 * p.num_kv_heads; j += 4) {
-    if (j & 1)
-      append_v_tile<D>(p, win, blk, j >> 1, lane);
+  const int tasks = n * heads * 2;
+  for (int j = wave; j < tasks; j += 4) {
+    const int c = j / (2 * heads), rest = j - c * 2 * heads, h = h0 + (rest >> 1);
+    if (foreign[c] || h >= p.num_kv_heads) continue;
+    if (rest & 1)
+      append_v_tile<D>(p, win[c], cand[c], h, lane);
     else
-      append_k_tile<D>(p, win, blk, j >> 1, lane);
+      append_k_tile<D>(p, win[c], cand[c], h, lane);
   }
 }
 
@@ -270,12 +376,22 @@ __global__ __launch_bounds__(256) void fca_gather_block_kernel(BlockCacheParams 
 
 hipError_t launch_append_block(const BlockCacheParams& p, hipStream_t stream) {
   if (p.num_tokens == 0) return hipSuccess;
+  // Windows: at most 128 of them up to their largest size (few workgroups look at all the slots);
+  // KV heads: as many groups as bring the launch to about 1024 workgroups.
+  int window = 1;
+  while (window < kMaxWindow && (p.num_tokens + window - 1) / window > 128) window *= 2;
+  const int windows = (p.num_tokens + window - 1) / window;
+  int groups = (1024 + windows - 1) / windows;
+  if (groups > p.num_kv_heads) groups = p.num_kv_heads;
+  const int heads = (p.num_kv_heads + groups - 1) / groups;
+  groups = (p.num_kv_heads + heads - 1) / heads;
+  const dim3 grid(windows * groups);
   if (p.head_dim == 64)
-    hipLaunchKernelGGL(fca_append_block_kernel<64>, dim3(p.num_tokens), dim3(256), 0, stream, p);
+    hipLaunchKernelGGL(fca_append_block_kernel<64>, grid, dim3(256), 0, stream, p, window, heads, groups);
   else if (p.head_dim == 128)
-    hipLaunchKernelGGL(fca_append_block_kernel<128>, dim3(p.num_tokens), dim3(256), 0, stream, p);
+    hipLaunchKernelGGL(fca_append_block_kernel<128>, grid, dim3(256), 0, stream, p, window, heads, groups);
   else
-    hipLaunchKernelGGL(fca_append_block_kernel<256>, dim3(p.num_tokens), dim3(256), 0, stream, p);
+    hipLaunchKernelGGL(fca_append_block_kernel<256>, grid, dim3(256), 0, stream, p, window, heads, groups);
   return hipGetLastError();
 }
 

@@ -24,7 +24,8 @@ ITEM_INTS = 8
 
 
 def _stream_ptr(device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    # (the handle itself; building a Stream object around it takes several microseconds a call)
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if device.index is None else device.index)
 
 
 @dataclasses.dataclass
