@@ -49,10 +49,20 @@ __device__ inline i32x4 first_codes(i32x4 raw, int n) {
   }
   return raw;
 }
-// The codes without those that are NaN; `found` collects where there were any.
-__device__ inline i32x4 without_nans(i32x4 raw, int& found) {
+// The same for a lane's own eight codes.
+__device__ inline i32x2 first_codes(i32x2 w, int n) {
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
+  for (int j = 0; j < 2; ++j) {
+    const int k = n - 4 * j;
+    w[j] &= k >= 4 ? -1 : k <= 0 ? 0 : (int)((1u << (8 * k)) - 1);
+  }
+  return w;
+}
+// The codes without those that are NaN; `found` collects where there were any.
+template <class V>
+__device__ inline V without_nans(V raw, int& found) {
+#pragma unroll
+  for (int j = 0; j < (int)(sizeof(V) / 4); ++j) {
     const int bad = (int)nan_bytes((unsigned)raw[j]);
     raw[j] &= ~bad;
     found |= bad;

@@ -84,10 +84,12 @@ __global__ __launch_bounds__(128, 2) void fca_attend_block_wide_kernel(AttendPar
   char* strip = strips[wave];
   const unsigned ring_lds = lds_address(&ring[0][0]);
 
-  // row `tile_row` of the stacked query tile is (member tile_row / G, head tile_row % G)
-  const int row_tile = Tune::kChannels ? 0 : wave;
-  const int tile_row = row_tile * 32 + m;
-  const int row_member = tile_row / G, row_head = tile_row - row_member * G;
+  // Row `row_tile * 32 + m` of the stacked query tile is (member row / G, head row % G).  Which wave
+  // takes which row tile changes from item to item: an item of 32 rows or fewer has work for one of
+  // the two, and that must not always be a wave on the same SIMD.
+  auto tile_of = [&](int round) { return Tune::kChannels ? 0 : (wave + round + me) & 1; };
+  const int member_of[2] = {m / G, (32 + m) / G};
+  const int head_of[2] = {m - member_of[0] * G, 32 + m - member_of[1] * G};
   const int channel0 = Tune::kChannels ? wave * Tune::kWaveD : 0;  // first output channel of this wave
   // MFMA row m carries the token whose index has bits 2 and 3 of m swapped: the score accumulator then
   // holds, per lane half, tokens 8h..8h+7 of each block in register order.
@@ -121,11 +123,13 @@ __global__ __launch_bounds__(128, 2) void fca_attend_block_wide_kernel(AttendPar
   auto tiles_of = [](const Item& x) { return (x.tok_len + kTile - 1) / kTile; };
   // one block id of the chunk per lane (a chunk has at most 64 blocks) and the member sequence of this
   // lane's query row
-  auto load_lane_meta = [&](const Item& x, int& blk, int& seq) {
+  auto load_lane_meta = [&](const Item& x, int row_tile, int& blk, int& seq) {
+    const int row_member = row_tile ? member_of[1] : member_of[0];
     blk = p.block_table[(int64_t)x.rep * p.bt_stride + x.blk_start + min(lane, blocks_of(x) - 1)];
     seq = meta[p.off_members + x.members + (row_member < x.mcnt ? row_member : 0)];
   };
-  auto load_q = [&](bf16x8 (&q)[KS], const Item& x, int seq) {
+  auto load_q = [&](bf16x8 (&q)[KS], const Item& x, int row_tile, int seq) {
+    const int row_member = row_tile ? member_of[1] : member_of[0], row_head = row_tile ? head_of[1] : head_of[0];
     const bool live = row_member < x.mcnt;
     const __bf16* qp = reinterpret_cast<const __bf16*>(p.q) + (int64_t)seq * p.q_seq_stride + (int64_t)(x.kvh * G + row_head) * p.q_head_stride;
 #pragma unroll
@@ -166,10 +170,10 @@ __global__ __launch_bounds__(128, 2) void fca_attend_block_wide_kernel(AttendPar
   // ---- set-up: records of the first three items, everything else of the first two
   Item cur = arrived(load_record(ticket(0))), nxt = arrived(load_record(ticket(1))), third = arrived(load_record(ticket(2)));
   int my_blk, a_blk, seq, a_seq;
-  load_lane_meta(cur, my_blk, seq);
-  load_lane_meta(nxt, a_blk, a_seq);
+  load_lane_meta(cur, tile_of(0), my_blk, seq);
+  load_lane_meta(nxt, tile_of(1), a_blk, a_seq);
   bf16x8 qreg[KS], nq[Tune::kEarlyQ ? KS : 1];
-  load_q(qreg, cur, seq);
+  load_q(qreg, cur, tile_of(0), seq);
   float2 my_scale = scales[(int64_t)my_blk * Hkv + cur.kvh];
   // Items take at least kAhead places in the stream of tiles (a short one repeats its last tile, which
   // nobody attends again), so that the ring never runs further ahead than into the next item.
@@ -180,9 +184,9 @@ __global__ __launch_bounds__(128, 2) void fca_attend_block_wide_kernel(AttendPar
     // ---- a step for each of the items ahead: query rows and scales of the next, block ids and members
     // of the one after it, record of the third
     int b_blk, b_seq;
-    load_lane_meta(third, b_blk, b_seq);
+    load_lane_meta(third, tile_of(round + 2), b_blk, b_seq);
     const RawItem fourth = load_record(ticket(round + 3));
-    if constexpr (Tune::kEarlyQ) load_q(nq, nxt, a_seq);
+    if constexpr (Tune::kEarlyQ) load_q(nq, nxt, tile_of(round + 1), a_seq);
     const float2 next_scale = scales[(int64_t)a_blk * Hkv + nxt.kvh];
     // Query rows fetched late have to be here before the loop over the tiles: a wait for them inside it
     // would also wait, every tile, for the requests the compiler does not know of.
@@ -196,7 +200,9 @@ __global__ __launch_bounds__(128, 2) void fca_attend_block_wide_kernel(AttendPar
     const int ntiles = tiles_of(cur), last = ntiles - 1, a_last = tiles_of(nxt) - 1;
     const int nfull = (tok_len - (sees > 0 ? 1 : 0)) / kTile;
     const int places = max(ntiles, kAhead);
-    const bool has_rows = Tune::kChannels || wave == 0 || mcnt * G > 32;
+    const int row_tile = tile_of(round);
+    const int row_member = row_tile ? member_of[1] : member_of[0], row_head = row_tile ? head_of[1] : head_of[0];
+    const bool has_rows = row_tile == 0 || mcnt * G > 32;
     const float ks_lane = my_scale.x * (p.scale * kLog2e);  // K scale of the lane's block, log2 domain
 
     f32x16 acc[NDB];
@@ -217,15 +223,29 @@ __global__ __launch_bounds__(128, 2) void fca_attend_block_wide_kernel(AttendPar
         ks[blk] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(ks_lane), b));
         vs[blk] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(my_scale.y), b));
       }
+      // (the fences keep reads of LDS together in front of the arithmetic they feed, V's in front of the
+      // softmax: left alone the compiler reads one piece, waits for it, and reads the next)
+      i32x4 kw[NK];
+      i32x2 vw[2][NDB];
+#pragma unroll
+      for (int i = 0; i < NK; ++i) kw[i] = tile[64 * i];
+      __builtin_amdgcn_sched_barrier(0);
       f32x16 sr;
 #pragma unroll
       for (int r = 0; r < 16; ++r) sr[r] = 0.f;
 #pragma unroll
-      for (int i = 0; i < KS; i += 2) {
-        const i32x4 w = tile[64 * (i >> 1)];
-        sr = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fp8x8_to_bf16(w[0], w[1]), qreg[i], sr, 0, 0, 0);
-        sr = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fp8x8_to_bf16(w[2], w[3]), qreg[i + 1], sr, 0, 0, 0);
+      for (int i = 0; i < NK; ++i) {
+        sr = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fp8x8_to_bf16(kw[i][0], kw[i][1]), qreg[2 * i], sr, 0, 0, 0);
+        sr = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fp8x8_to_bf16(kw[i][2], kw[i][3]), qreg[2 * i + 1], sr, 0, 0, 0);
       }
+      // codes of tokens 8h..8h+7 of channel 32 * db + m: its 16 tokens lie together in a piece of 64 channels
+      const char* values = &ring[slot][0] + (NK + 2 * (channel0 / 64)) * 1024 + m * 16 + h * 8;
+#pragma unroll
+      for (int db = 0; db < NDB; ++db)
+#pragma unroll
+        for (int blk = 0; blk < 2; ++blk)
+          vw[blk][db] = *reinterpret_cast<const i32x2*>(values + (2 * (db >> 1) + blk) * 1024 + (db & 1) * 512);
+      __builtin_amdgcn_sched_barrier(0);
       // register r holds token 16 * (r / 8) + 8 * h + r % 8 of the tile, for this lane's query row
       if constexpr (RAGGED) {
         const int lim = (sees > 0 ? min(tok_len, sees + row_member) : tok_len) - tok0 - 8 * h;
@@ -266,24 +286,19 @@ __global__ __launch_bounds__(128, 2) void fca_attend_block_wide_kernel(AttendPar
         pb[r >> 3][r & 7] = (__bf16)(e * vs[r >> 3]);
       }
       lrow += sum;
-      const i32x4* values = tile + 64 * (NK + 2 * (channel0 / 64));
       // (`run`: the last tile of a query run, whose rows see different numbers of its tokens)
       const bool run = RAGGED && sees > 0;
       int nans = 0;
 #pragma unroll
       for (int blk = 0; blk < 2; ++blk)
 #pragma unroll
-        for (int pair = 0; pair < NDB / 2; ++pair) {
-          i32x4 raw = values[64 * (2 * pair + blk)];
+        for (int db = 0; db < NDB; ++db) {
+          i32x2 w = vw[blk][db];
           if constexpr (RAGGED) {
-            raw = first_codes(raw, tok_len - (tok0 + 16 * blk));
-            if (run) raw = without_nans(raw, nans);
+            w = first_codes(w, tok_len - (tok0 + 16 * blk + 8 * h));
+            if (run) w = without_nans(w, nans);
           }
-#pragma unroll
-          for (int db = 2 * pair; db < 2 * pair + 2; ++db) {
-            const i32x2 w = value_codes(raw, db);
-            acc[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fp8x8_to_bf16(w[0], w[1]), pb[blk], acc[db], 0, 0, 0);
-          }
+          acc[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fp8x8_to_bf16(w[0], w[1]), pb[blk], acc[db], 0, 0, 0);
         }
       // A NaN among the values of such a tile must not reach the rows that do not see its token (0 * NaN),
       // so it was left out of the product.  Where a row does see one, the product of (huge where the
@@ -299,7 +314,7 @@ __global__ __launch_bounds__(128, 2) void fca_attend_block_wide_kernel(AttendPar
             for (int r = 0; r < 16; ++r) hit[r] = 0.f;
 #pragma unroll
             for (int blk = 0; blk < 2; ++blk) {
-              const i32x2 w = value_codes(first_codes(values[64 * (2 * (db >> 1) + blk)], tok_len - (tok0 + 16 * blk)), db);
+              const i32x2 w = first_codes(vw[blk][db], tok_len - (tok0 + 16 * blk + 8 * h));
               bf16x8 vis;
 #pragma unroll
               for (int k = 0; k < 8; ++k) vis[k] = (__bf16)(k + 16 * blk < seen ? kHuge : 0.f);
@@ -405,7 +420,7 @@ __global__ __launch_bounds__(128, 2) void fca_attend_block_wide_kernel(AttendPar
 #pragma unroll
       for (int i = 0; i < KS; ++i) qreg[i] = nq[i];
     } else {
-      load_q(qreg, nxt, a_seq);
+      load_q(qreg, nxt, tile_of(round + 1), a_seq);
     }
     my_scale = next_scale;
     my_blk = a_blk, seq = a_seq, a_blk = b_blk, a_seq = b_seq;
