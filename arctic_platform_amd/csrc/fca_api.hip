@@ -152,7 +152,7 @@ int run_attend(const fca_plan* p, const fca_tensors* t, void* meta, void* po, fl
 }
 
 int run_merge(const fca_plan* p, const void* meta, const void* po, const float* pl, void* out, int64_t oss, int64_t ohs,
-              int32_t out_dtype, float* lse, void* stream, bool partial_f32 = false) {
+              int32_t out_dtype, float* lse, void* stream, bool partial_f32 = false, bool block_scaled = false) {
   if (int rc = check_plan(p)) return rc;
   if (!meta || !po || !pl || !out) return fail(FCA_ERR_INVALID_ARG, "metadata, partials and out must be non-NULL");
   if (out_dtype != FCA_BF16 && out_dtype != FCA_F32)
@@ -180,7 +180,12 @@ int run_merge(const fca_plan* p, const void* meta, const void* po, const float* 
   // whole 16-byte stores when every 8-channel group of out is 16-byte aligned
   const int64_t esz = out_dtype == FCA_F32 ? 4 : 2;
   m.vector_out = !(reinterpret_cast<uintptr_t>(out) & 15) && (oss * esz) % 16 == 0 && (ohs * esz) % 16 == 0;
-  hipError_t e = fca::launch_merge(m, static_cast<hipStream_t>(stream));
+  // Few rows that can have many partials, after attention over a block-scaled cache: a workgroup each
+  // (32 rows of 128 partials 12 -> 6 us; 4096 rows of 36 would take 16.6 us against 14.1, so from
+  // four rows per CU on a wave or less each; the other caches keep their order of summation).
+  const bool few_long = block_scaled && m.max_partials >= 16 && (int64_t)m.num_seqs * m.num_q_heads <= 1024;
+  hipError_t e = few_long ? fca::launch_merge_long(m, static_cast<hipStream_t>(stream))
+                          : fca::launch_merge(m, static_cast<hipStream_t>(stream));
   return e == hipSuccess ? FCA_OK : hip_fail(e, "merge launch");
 }
 
@@ -323,7 +328,7 @@ int fca_decode_step(const fca_plan* plan, const fca_tensors* t, void* meta_dev, 
                     int32_t out_dtype, float* lse_dev, void* stream) {
   if (int rc = run_attend(plan, t, meta_dev, partial_out_dev, partial_lse_dev, 0, stream, true)) return rc;
   return run_merge(plan, meta_dev, partial_out_dev, partial_lse_dev, out_dev, out_seq_stride, out_head_stride, out_dtype,
-                   lse_dev, stream, t->kv_dtype == FCA_F32);
+                   lse_dev, stream, t->kv_dtype == FCA_F32, t->kv_dtype == FCA_FP8_E4M3_BLOCK);
 }
 
 }  // extern "C"
@@ -380,7 +385,7 @@ int fca_decode_step_static(const fca_plan* plan, const fca_tensors* t, void* met
   float* partial_lse = reinterpret_cast<float*>(base + lse_at);
   if (int rc = run_attend(plan, t, meta_dev, partial_out, partial_lse, 0, stream, true)) return rc;
   return run_merge(plan, meta_dev, partial_out, partial_lse, out_dev, out_seq_stride, out_head_stride, out_dtype, lse_dev,
-                   stream, t->kv_dtype == FCA_F32);
+                   stream, t->kv_dtype == FCA_F32, t->kv_dtype == FCA_FP8_E4M3_BLOCK);
 }
 
 static int cache_rows(bool gather, const void* key_dev, const void* value_dev, int64_t token_stride, int64_t head_stride,
@@ -446,8 +451,8 @@ static int cache_rows_block(bool gather, const void* key_dev, const void* value_
   if (num_tokens < 0 || num_kv_heads < 1) return fail(FCA_ERR_INVALID_ARG, "num_tokens must be >= 0 and num_kv_heads >= 1");
   if (head_dim != 64 && head_dim != 128 && head_dim != 256)
     return fail(FCA_ERR_UNSUPPORTED, "head_dim %d is not supported (64, 128 or 256)", head_dim);
-  if (num_blocks < 0 || num_blocks > 0x7fffffffLL)
-    return fail(FCA_ERR_INVALID_ARG, "num_blocks %lld must lie in [0, 2^31)", (long long)num_blocks);
+  if (num_blocks < 1 || num_blocks > 0x7fffffffLL)
+    return fail(FCA_ERR_INVALID_ARG, "num_blocks %lld must lie in [1, 2^31)", (long long)num_blocks);
   if (num_tokens == 0) return FCA_OK;
   if (!key_dev || !value_dev || !slot_mapping_dev || !k_cache_dev || !v_cache_dev || !block_scales_dev)
     return fail(FCA_ERR_INVALID_ARG, "key, value, slot_mapping, the cache planes and block_scales must be non-NULL");

@@ -50,6 +50,7 @@ struct BlockCacheParams {
 };
 hipError_t launch_append_block(const BlockCacheParams& p, hipStream_t stream);
 hipError_t launch_gather_block(const BlockCacheParams& p, hipStream_t stream);
+hipError_t launch_merge_long(const MergeParams& p, hipStream_t stream);
 hipError_t launch_attend_block(const AttendParams& p, const fca_plan& plan, int max_workgroups, hipStream_t stream);
 
 }  // namespace fca

@@ -104,56 +104,6 @@ __device__ inline ScaleStep step_scale(float* at, float was, unsigned lane_amax,
   return s;
 }
 
-// `win`: the call's token at every offset of the block, -1 = none.
-template <int D>
-__device__ inline void append_k_tile(const BlockCacheParams& p, const int* win, int64_t blk, int h, int lane) {
-  constexpr int U = D / 64;  // 16-byte units of the tile per lane
-  const int tok = lane & 15;
-  const int t = win[tok];
-  float* at = p.scales + (blk * p.num_kv_heads + h) * 2;
-  const float was = *at;  // (every lane has it before the reduction, lane 0 writes behind it)
-  char* tile = static_cast<char*>(p.k_cache) + blk * p.cache_block_stride + h * p.cache_head_stride;
-  const unsigned short* row = static_cast<const unsigned short*>(p.key) + (int64_t)t * p.token_stride + (int64_t)h * p.head_stride;
-  unsigned in[U * 8];
-  union Codes {
-    int4 raw;
-    unsigned w[4];
-  } out[U];
-#pragma unroll
-  for (int i = 0; i < U; ++i) {
-    const int c = (lane >> 4) + 4 * i;
-    int4 x0 = make_int4(0, 0, 0, 0), x1 = x0;
-    if (t >= 0) {
-      x0 = *reinterpret_cast<const int4*>(row + 16 * c);
-      x1 = *reinterpret_cast<const int4*>(row + 16 * c + 8);
-    } else {
-      out[i].raw = *reinterpret_cast<const int4*>(tile + (c * kBlock + tok) * 16);
-    }
-    in[8 * i] = x0.x, in[8 * i + 1] = x0.y, in[8 * i + 2] = x0.z, in[8 * i + 3] = x0.w;
-    in[8 * i + 4] = x1.x, in[8 * i + 5] = x1.y, in[8 * i + 6] = x1.z, in[8 * i + 7] = x1.w;
-  }
-  bool special;
-  const unsigned amax = lane_max(in, special);
-  const ScaleStep s = step_scale(at, was, amax, special, win[0] >= 0, lane);
-  if (t < 0 && !s.grown) return;
-#pragma unroll
-  for (int i = 0; i < U; ++i) {
-    const int c = (lane >> 4) + 4 * i;
-    if (t >= 0) {
-#pragma unroll
-      for (int d = 0; d < 4; ++d) {
-        const unsigned lo = in[8 * i + 2 * d], hi = in[8 * i + 2 * d + 1];
-        const float x0 = bf16_low(lo) * s.inv, x1 = bf16_high(lo) * s.inv, x2 = bf16_low(hi) * s.inv, x3 = bf16_high(hi) * s.inv;
-        out[i].w[d] = s.special ? e4m3_codes(x0, x1, x2, x3) : e4m3_codes_of_small(x0, x1, x2, x3);
-      }
-    } else {
-#pragma unroll
-      for (int d = 0; d < 4; ++d) out[i].w[d] = rescaled_codes(out[i].w[d], s.ratio);
-    }
-    *reinterpret_cast<int4*>(tile + (c * kBlock + tok) * 16) = out[i].raw;
-  }
-}
-
 // CH adjacent bf16 numbers (an element access of 2, 4 or 8 bytes) as dwords.
 template <int CH>
 __device__ inline void load_channels(const unsigned short* from, unsigned (&w)[(CH + 1) / 2]) {
@@ -167,39 +117,76 @@ __device__ inline void load_channels(const unsigned short* from, unsigned (&w)[(
   }
 }
 
+// K and V of one block and KV head; all loads of both are in flight together.  `win`: the call's token at
+// every offset of the block, -1 = none.
 template <int D>
-__device__ inline void append_v_tile(const BlockCacheParams& p, const int* win, int64_t blk, int h, int lane) {
-  constexpr int CH = D / 64;  // adjacent channels per lane
-  constexpr int W = (CH + 1) / 2;
-  float* at = p.scales + (blk * p.num_kv_heads + h) * 2 + 1;
-  const float was = *at;
-  char* tile = static_cast<char*>(p.v_cache) + blk * p.cache_block_stride + h * p.cache_head_stride + lane * CH * kBlock;
-  const unsigned short* rows = static_cast<const unsigned short*>(p.value) + (int64_t)h * p.head_stride + lane * CH;
-  const int mine = win[lane & 15];
-  const unsigned live = (unsigned)(__ballot(mine >= 0) & 0xffff);
+__device__ inline void append_tiles(const BlockCacheParams& p, const int* win, int64_t blk, int h, int lane) {
+  constexpr int U = D / 64;            // K: 16-byte units of the tile per lane
+  constexpr int CH = D / 64;           // V: adjacent channels per lane
+  constexpr int W = (CH + 1) / 2;      // ... as dwords
   union Codes {
     int4 raw;
     unsigned w[4];
-  } old[CH];
-  if (live != 0xffff) {
+  };
+  const int tok = lane & 15;
+  const int mine = win[tok];
+  const unsigned live = (unsigned)(__ballot(mine >= 0) & 0xffff);
+  const bool begins = live & 1;
+  float* at = p.scales + (blk * p.num_kv_heads + h) * 2;
+  const float k_was = at[0], v_was = at[1];  // (every lane has them before the reductions, lane 0 writes behind those)
+  const int64_t tile_at = blk * p.cache_block_stride + h * p.cache_head_stride;
+  char* k_tile = static_cast<char*>(p.k_cache) + tile_at;
+  char* v_tile = static_cast<char*>(p.v_cache) + tile_at + lane * CH * kBlock;
+  const unsigned short* k_row = static_cast<const unsigned short*>(p.key) + (int64_t)mine * p.token_stride + (int64_t)h * p.head_stride;
+  const unsigned short* v_rows = static_cast<const unsigned short*>(p.value) + (int64_t)h * p.head_stride + lane * CH;
+
+  unsigned k_in[U * 8];
+  Codes k_out[U], v_out[CH];
 #pragma unroll
-    for (int ch = 0; ch < CH; ++ch) old[ch].raw = *reinterpret_cast<const int4*>(tile + ch * kBlock);
-  } else {
-#pragma unroll
-    for (int ch = 0; ch < CH; ++ch) old[ch].raw = make_int4(0, 0, 0, 0);
+  for (int i = 0; i < U; ++i) {
+    const int c = (lane >> 4) + 4 * i;
+    int4 x0 = make_int4(0, 0, 0, 0), x1 = x0;
+    if (mine >= 0) {
+      x0 = *reinterpret_cast<const int4*>(k_row + 16 * c);
+      x1 = *reinterpret_cast<const int4*>(k_row + 16 * c + 8);
+    } else {
+      k_out[i].raw = *reinterpret_cast<const int4*>(k_tile + (c * kBlock + tok) * 16);
+    }
+    k_in[8 * i] = x0.x, k_in[8 * i + 1] = x0.y, k_in[8 * i + 2] = x0.z, k_in[8 * i + 3] = x0.w;
+    k_in[8 * i + 4] = x1.x, k_in[8 * i + 5] = x1.y, k_in[8 * i + 6] = x1.z, k_in[8 * i + 7] = x1.w;
   }
-  unsigned in[kBlock * W];
+#pragma unroll
+  for (int ch = 0; ch < CH; ++ch)
+    v_out[ch].raw = live != 0xffff ? *reinterpret_cast<const int4*>(v_tile + ch * kBlock) : make_int4(0, 0, 0, 0);
+  unsigned v_in[kBlock * W];
 #pragma unroll
   for (int k = 0; k < kBlock; ++k) {
     const int t = __builtin_amdgcn_readlane(mine, k);
     unsigned w[W] = {};
-    if (t >= 0) load_channels<CH>(rows + (int64_t)t * p.token_stride, w);
+    if (t >= 0) load_channels<CH>(v_rows + (int64_t)t * p.token_stride, w);
 #pragma unroll
-    for (int i = 0; i < W; ++i) in[k * W + i] = w[i];
+    for (int i = 0; i < W; ++i) v_in[k * W + i] = w[i];
   }
-  bool special;
-  const unsigned amax = lane_max(in, special);
-  const ScaleStep s = step_scale(at, was, amax, special, live & 1, lane);
+
+  bool k_special, v_special;
+  const unsigned k_amax = lane_max(k_in, k_special), v_amax = lane_max(v_in, v_special);
+  const ScaleStep ks = step_scale(at, k_was, k_amax, k_special, begins, lane);
+  const ScaleStep vs = step_scale(at + 1, v_was, v_amax, v_special, begins, lane);
+
+  if (mine >= 0 || ks.grown) {
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const int c = (lane >> 4) + 4 * i;
+#pragma unroll
+      for (int d = 0; d < 4; ++d) {
+        const unsigned lo = k_in[8 * i + 2 * d], hi = k_in[8 * i + 2 * d + 1];
+        const float x0 = bf16_low(lo) * ks.inv, x1 = bf16_high(lo) * ks.inv, x2 = bf16_low(hi) * ks.inv, x3 = bf16_high(hi) * ks.inv;
+        if (mine < 0) k_out[i].w[d] = rescaled_codes(k_out[i].w[d], ks.ratio);
+        else k_out[i].w[d] = ks.special ? e4m3_codes(x0, x1, x2, x3) : e4m3_codes_of_small(x0, x1, x2, x3);
+      }
+      *reinterpret_cast<int4*>(k_tile + (c * kBlock + tok) * 16) = k_out[i].raw;
+    }
+  }
 #pragma unroll
   for (int ch = 0; ch < CH; ++ch) {
 #pragma unroll
@@ -207,17 +194,17 @@ __device__ inline void append_v_tile(const BlockCacheParams& p, const int* win, 
       float x[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const unsigned w = in[(4 * d + e) * W + ch / 2];
-        x[e] = (ch & 1 ? bf16_high(w) : bf16_low(w)) * s.inv;
+        const unsigned w = v_in[(4 * d + e) * W + ch / 2];
+        x[e] = (ch & 1 ? bf16_high(w) : bf16_low(w)) * vs.inv;
       }
-      const unsigned q = s.special ? e4m3_codes(x[0], x[1], x[2], x[3]) : e4m3_codes_of_small(x[0], x[1], x[2], x[3]);
+      const unsigned q = vs.special ? e4m3_codes(x[0], x[1], x[2], x[3]) : e4m3_codes_of_small(x[0], x[1], x[2], x[3]);
       // bytes of the call's tokens (the same in every lane)
       const unsigned four = (live >> (4 * d)) & 15;
       const unsigned fresh = ((four & 1) | (four & 2) << 7 | (four & 4) << 14 | (four & 8) << 21) * 0xffu;
-      const unsigned kept = s.grown ? rescaled_codes(old[ch].w[d], s.ratio) : old[ch].w[d];
-      old[ch].w[d] = (q & fresh) | (kept & ~fresh);
+      const unsigned kept = vs.grown ? rescaled_codes(v_out[ch].w[d], vs.ratio) : v_out[ch].w[d];
+      v_out[ch].w[d] = (q & fresh) | (kept & ~fresh);
     }
-    *reinterpret_cast<int4*>(tile + ch * kBlock) = old[ch].raw;
+    *reinterpret_cast<int4*>(v_tile + ch * kBlock) = v_out[ch].raw;
   }
 }
 
@@ -257,129 +244,147 @@ __global__ __launch_bounds__(256) void fca_append_block_kernel(BlockCacheParams 
   __syncthreads();
   const int n = num_cand;
   if (n == 0) return;
-  // (four slots per thread and trip: their loads are in flight together)
-  for (int base = 0; base < p.num_tokens; base += 1024) {
-    int blk[4], off[4];
+  // (kScan slots per thread and trip, whose loads are in flight together)
+  constexpr int kScan = 16;
+  for (int base = 0; base < p.num_tokens; base += 256 * kScan) {
+    int64_t slots[kScan];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
+    for (int k = 0; k < kScan; ++k) {
       const int t = base + 256 * k + tid;
-      int64_t slot = -1;
-      if (t < p.num_tokens) slot = p.slot_mapping[t];
-      blk[k] = slot >= 0 && slot < end ? (int)(slot / kBlock) : -1;
-      off[k] = (int)(slot & (kBlock - 1));
+      slots[k] = t < p.num_tokens ? p.slot_mapping[t] : -1;
     }
-    for (int c = 0; c < n; ++c) {
-      const int mine = cand[c];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        if (blk[k] != mine) continue;
-        const int t = base + 256 * k + tid;
+    for (int k = 0; k < kScan; ++k) {
+      if (base + 256 * k >= p.num_tokens) break;
+      const int blk = slots[k] >= 0 && slots[k] < end ? (int)(slots[k] / kBlock) : -1;
+      const int t = base + 256 * k + tid;
+      for (int c = 0; c < n; ++c) {
+        if (blk != cand[c]) continue;
         if (t < t0) foreign[c] = 1;
-        else atomicMax(&win[c][off[k]], t);
+        else atomicMax(&win[c][(int)slots[k] & (kBlock - 1)], t);
       }
     }
   }
   __syncthreads();
-  const int tasks = n * heads * 2;
+  const int tasks = n * heads;
   for (int j = wave; j < tasks; j += 4) {
-    const int c = j / (2 * heads), rest = j - c * 2 * heads, h = h0 + (rest >> 1);
+    const int c = j / heads, h = h0 + j - c * heads;
     if (foreign[c] || h >= p.num_kv_heads) continue;
-    if (rest & 1)
-      append_v_tile<D>(p, win[c], cand[c], h, lane);
-    else
-      append_k_tile<D>(p, win[c], cand[c], h, lane);
+    append_tiles<D>(p, win[c], cand[c], h, lane);
   }
 }
 
 // Reading back: row t = codes at slot_mapping[t] times their block's scales, rounded to bf16 (exact
 // for the writer's scales, short of bf16's own range); a negative slot, or one past the cache, gives
-// zeros.  A wave takes 16 tokens of one head and plane.
+// zeros.  A wave takes 16 tokens of one head and plane.  Of K a lane converts 16-byte units, as in
+// the writer.  Of V a lane holds whole channels of one block at a time and writes every token of the
+// group that lies in the block, offset by offset, so that a code's place in its register is known at
+// compile time and a row leaves as one contiguous store of the wave; a run of consecutive tokens
+// touches at most two blocks, both fetched in advance.
 template <int D>
 __global__ __launch_bounds__(256) void fca_gather_block_kernel(BlockCacheParams p) {
-  const int lane = threadIdx.x & 63;
-  const int64_t task = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  constexpr int CH = D / 64;  // adjacent channels per lane (V)
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t task = (int64_t)blockIdx.x * 4 + wave;
   const int64_t group = task / (2 * p.num_kv_heads);
   const int j = (int)(task - group * 2 * p.num_kv_heads), h = j >> 1;
-  const int64_t t0 = group * 16;
+  const int64_t t0 = group * kBlock;
   if (t0 >= p.num_tokens) return;
-  const int64_t end = p.num_blocks * kBlock;
   const int64_t t = t0 + (lane & 15);
-  int64_t slot = t < p.num_tokens ? p.slot_mapping[t] : -1;
-  if (slot >= end) slot = -1;
-  const int64_t blk = slot < 0 ? 0 : slot / kBlock;
-  const int off = slot < 0 ? 0 : (int)(slot % kBlock);
-  const float scale = slot < 0 ? 0.f : p.scales[(blk * p.num_kv_heads + h) * 2 + (j & 1)];
+  const int64_t slot = t < p.num_tokens ? p.slot_mapping[t] : -1;
+  const bool live = slot >= 0 && slot < p.num_blocks * kBlock;
+  const int blk = live ? (int)(slot / kBlock) : -1, off = live ? (int)(slot % kBlock) : 0;
+  const float scale = live ? p.scales[((int64_t)blk * p.num_kv_heads + h) * 2 + (j & 1)] : 0.f;
   if ((j & 1) == 0) {
     constexpr int U = D / 64;
     if (t >= p.num_tokens) return;
-    const char* tile = static_cast<const char*>(p.k_cache) + blk * p.cache_block_stride + h * p.cache_head_stride;
+    const char* tile = static_cast<const char*>(p.k_cache) + (int64_t)max(blk, 0) * p.cache_block_stride + h * p.cache_head_stride;
     __hip_bfloat16* row = static_cast<__hip_bfloat16*>(const_cast<void*>(p.key)) + t * p.token_stride + (int64_t)h * p.head_stride;
+    int4 q[U];
+#pragma unroll
+    for (int i = 0; i < U; ++i)
+      q[i] = live ? *reinterpret_cast<const int4*>(tile + (((lane >> 4) + 4 * i) * kBlock + off) * 16) : make_int4(0, 0, 0, 0);
 #pragma unroll
     for (int i = 0; i < U; ++i) {
       const int c = (lane >> 4) + 4 * i;
-      union {
-        int4 raw;
-        unsigned w[4];
-      } q;
+      const int w[4] = {q[i].x, q[i].y, q[i].z, q[i].w};
       union {
         int4 raw[2];
         __hip_bfloat16 x[16];
       } o;
-      if (slot >= 0) {
-        q.raw = *reinterpret_cast<const int4*>(tile + (c * kBlock + off) * 16);
 #pragma unroll
-        for (int e = 0; e < 16; ++e)
-          o.x[e] = __float2bfloat16(__builtin_amdgcn_cvt_f32_fp8((int)(q.w[e >> 2] >> (8 * (e & 3))), 0) * scale);
-      } else {
-        o.raw[0] = o.raw[1] = make_int4(0, 0, 0, 0);
+      for (int d = 0; d < 4; ++d) {
+        const auto a = __builtin_amdgcn_cvt_pk_f32_fp8(w[d], false), b = __builtin_amdgcn_cvt_pk_f32_fp8(w[d], true);
+        o.x[4 * d] = __float2bfloat16(a[0] * scale), o.x[4 * d + 1] = __float2bfloat16(a[1] * scale);
+        o.x[4 * d + 2] = __float2bfloat16(b[0] * scale), o.x[4 * d + 3] = __float2bfloat16(b[1] * scale);
       }
       reinterpret_cast<int4*>(row + 16 * c)[0] = o.raw[0];
       reinterpret_cast<int4*>(row + 16 * c)[1] = o.raw[1];
     }
-  } else {
-    constexpr int CH = D / 64;
-    struct alignas(2 * CH) Piece {
-      __hip_bfloat16 x[CH];
-    };
-    union {
-      int4 raw;
-      unsigned w[4];
-    } q[CH];
-    int held = -1;  // token of the group whose block's codes are in q
-    for (int k = 0; k < 16 && t0 + k < p.num_tokens; ++k) {
-      const int64_t sk = __shfl(slot, k);
-      const float vs = __shfl(scale, k);
-      Piece o;
-      if (sk < 0) {
+    return;
+  }
+  struct alignas(2 * CH) Piece {
+    __hip_bfloat16 x[CH];
+  };
+  struct Codes {
+    int w[CH][4];
+  };
+  __hip_bfloat16* rows = static_cast<__hip_bfloat16*>(const_cast<void*>(p.value)) + t0 * p.token_stride + (int64_t)h * p.head_stride + lane * CH;
+  auto load = [&](int b) {
+    const char* tile = static_cast<const char*>(p.v_cache) + (int64_t)max(b, 0) * p.cache_block_stride + h * p.cache_head_stride;
+    Codes c;
 #pragma unroll
-        for (int ch = 0; ch < CH; ++ch) o.x[ch] = __float2bfloat16(0.f);
-      } else {
-        if (held < 0 || __shfl(blk, held) != sk / kBlock) {
-          held = k;
-          const char* tile = static_cast<const char*>(p.v_cache) + sk / kBlock * p.cache_block_stride + h * p.cache_head_stride;
-#pragma unroll
-          for (int ch = 0; ch < CH; ++ch) q[ch].raw = *reinterpret_cast<const int4*>(tile + (lane * CH + ch) * kBlock);
-        }
-        const int ok = (int)(sk % kBlock);
-#pragma unroll
-        for (int ch = 0; ch < CH; ++ch) {
-          const unsigned lo = ok & 4 ? q[ch].w[1] : q[ch].w[0], hi = ok & 4 ? q[ch].w[3] : q[ch].w[2];
-          const unsigned w = (ok & 8 ? hi : lo) >> (8 * (ok & 3));
-          o.x[ch] = __float2bfloat16(__builtin_amdgcn_cvt_f32_fp8((int)w, 0) * vs);
-        }
-      }
-      *reinterpret_cast<Piece*>(static_cast<__hip_bfloat16*>(const_cast<void*>(p.value)) + (t0 + k) * p.token_stride +
-                                (int64_t)h * p.head_stride + lane * CH) = o;
+    for (int ch = 0; ch < CH; ++ch) {
+      const int4 x = *reinterpret_cast<const int4*>(tile + (lane * CH + ch) * kBlock);
+      c.w[ch][0] = x.x, c.w[ch][1] = x.y, c.w[ch][2] = x.z, c.w[ch][3] = x.w;
     }
+    return c;
+  };
+  const int tokens = (int)min((int64_t)kBlock, (int64_t)p.num_tokens - t0);
+  const bool is_token = lane < tokens;
+  const int first = __builtin_amdgcn_readlane(blk, 0), last = __builtin_amdgcn_readlane(blk, tokens - 1);
+  const Codes ca = load(first), cb = load(last);  // (block 0 where there is none: its codes are not used)
+  unsigned todo = (unsigned)__ballot(is_token && blk >= 0);
+  const unsigned padding = (unsigned)__ballot(is_token && blk < 0);
+  // the tokens still to do that lie in block b, one per offset (of two with one slot the second waits)
+  auto write = [&](const Codes& c, int b) {
+    const bool here = ((todo >> (lane & 31)) & 1) && lane < kBlock && blk == b;
+    const float vs = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(scale), __builtin_ctzll(__ballot(here))));
+#pragma unroll
+    for (int o = 0; o < kBlock; ++o) {
+      const unsigned at = (unsigned)__ballot(here && off == o);
+      if (at == 0) continue;
+      const int k = __builtin_ctz(at);
+      todo &= ~(1u << k);
+      Piece x;
+#pragma unroll
+      for (int ch = 0; ch < CH; ++ch) {
+        const unsigned w = (unsigned)c.w[ch][o >> 2] >> (8 * (o & 3));
+        x.x[ch] = __float2bfloat16(__builtin_amdgcn_cvt_f32_fp8((int)w, 0) * vs);
+      }
+      *reinterpret_cast<Piece*>(rows + (int64_t)k * p.token_stride) = x;
+    }
+  };
+  if (first >= 0) write(ca, first);
+  if (todo != 0 && last >= 0 && last != first) write(cb, last);
+  while (todo != 0) {
+    const int b = __builtin_amdgcn_readlane(blk, __builtin_ctz(todo));
+    write(load(b), b);
+  }
+  for (unsigned left = padding; left != 0; left &= left - 1) {
+    Piece zero;
+#pragma unroll
+    for (int ch = 0; ch < CH; ++ch) zero.x[ch] = __float2bfloat16(0.f);
+    *reinterpret_cast<Piece*>(rows + (int64_t)__builtin_ctz(left) * p.token_stride) = zero;
   }
 }
 
 hipError_t launch_append_block(const BlockCacheParams& p, hipStream_t stream) {
   if (p.num_tokens == 0) return hipSuccess;
-  // Windows: at most 128 of them up to their largest size (few workgroups look at all the slots);
+  // Windows: at most 512 of them up to their largest size (few workgroups look at all the slots);
   // KV heads: as many groups as bring the launch to about 1024 workgroups.
   int window = 1;
-  while (window < kMaxWindow && (p.num_tokens + window - 1) / window > 128) window *= 2;
+  while (window < kMaxWindow && (p.num_tokens + window - 1) / window > 512) window *= 2;
   const int windows = (p.num_tokens + window - 1) / window;
   int groups = (1024 + windows - 1) / windows;
   if (groups > p.num_kv_heads) groups = p.num_kv_heads;

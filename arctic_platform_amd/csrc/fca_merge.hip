@@ -123,8 +123,11 @@ __global__ __launch_bounds__(kMergeThreads) void fca_merge_kernel(MergeParams p)
       }
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int j = 0; j < B; ++j)
+      for (int j = 0; j < B; ++j) {
+        // (a second partial carries a tag itself only where its row is no number, fca_attend_block.h)
+        if (rel[j] >= 0 && (__float_as_uint(bls[j][1]) & 0x007fffffu) != 0) stray = 1;
         take(rel[j] >= 0 ? bls[j][0] : -INFINITY, __uint_as_float(__float_as_uint(bls[j][1]) & 0xff800000u), bo[j]);
+      }
     }
   }
   // combine the shares: the same update with a whole running result in place of one partial

@@ -335,6 +335,25 @@ def test_attention_on_random_forests(gpu, case, levels):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("d,hq,hkv,rows,lens", [(64, 4, 1, 32, (1030, 0, 17)), (128, 4, 2, 64, (700, 533)), (256, 2, 1, 32, (560,)), (128, 8, 1, 32, (3000, 40, 2049))])
+@pytest.mark.parametrize("out_dtype", [torch.bfloat16, torch.float32])
+def test_attention_on_rows_of_many_partials(gpu, d, hq, hkv, rows, lens, out_dtype):
+    """Chunks of one tile: rows of up to 94 partials, next to short and empty ones."""
+    from arctic_platform_amd import build_forest_metadata, forest_cascade_decode
+
+    g = torch.Generator().manual_seed(len(lens) + d)
+    w = make_forest_workload("long", list(lens), [[i] for i in range(len(lens))], g, num_q_heads=hq, num_kv_heads=hkv, head_dim=d, kv_dtype=FP8, poison_unused=True)
+    scales = _random_scales(g, w.kv_cache, _used_blocks(w.block_table, w.seq_lens), powers=False)
+    md = build_forest_metadata(w.block_table.to(gpu), w.seq_lens.to(gpu), num_q_heads=hq, num_kv_heads=hkv, head_dim=d, chunk_tokens=32, rows_per_item=rows)
+    assert md.layout.max_partials >= 16
+    wide = torch.full((len(lens), hq, d + 8), 5.0, dtype=out_dtype).to(gpu)
+    out, lse = forest_cascade_decode(w.q.to(gpu), w.kv_cache.to(gpu), md, w.scale, out=wide[..., 4 : d + 4], block_scales=scales.to(gpu))
+    torch.cuda.synchronize()
+    assert (wide[..., :4] == 5).all() and (wide[..., d + 4 :] == 5).all()
+    _check_attention(out, lse, w.q, w.kv_cache, scales, w.block_table, range(len(lens)), list(lens), w.scale, f"lengths {lens}")
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("d,hq,hkv,rows,n", [(64, 8, 2, 32, 1), (128, 8, 2, 32, 1), (256, 4, 1, 32, 1), (128, 4, 4, 64, 16), (64, 4, 4, 64, 17), (128, 16, 2, 32, 31), (128, 16, 2, 32, 32), (128, 8, 8, 32, 33)])
 def test_attention_on_one_short_sequence(gpu, d, hq, hkv, rows, n):
     from arctic_platform_amd import build_forest_metadata, forest_cascade_decode

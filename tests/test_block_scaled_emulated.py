@@ -99,6 +99,36 @@ def test_query_runs_with_a_nan(emu, order, d, rows):  # noqa: F811
     _check_attention(torch.where(bad, ref.bfloat16(), out), lse, q, clean, scales, table, row_table, row_lens, 0.1, "query runs")
 
 
+@pytest.mark.parametrize("rows,hkv,max_len", [(32, 4, None), (64, 4, None), (32, 1, 2900)])
+def test_nan_keys_in_items_shared_by_two_waves(emu, rows, hkv, max_len):  # noqa: F811
+    """NaN keys all over long prompts and private parts: a row is NaN, log-sum-exp included, exactly where
+    it sees one, whichever wave of a pair attended the tile that holds it and whichever merge follows."""
+    hq, d, chunk = 4 * hkv, 128, 512
+    g = torch.Generator().manual_seed(77)
+    if max_len is None:
+        seg = [700 + 300 * i for i in range(6)] + [40 + 29 * i for i in range(18)]
+        paths = [[i // 3, 6 + i] for i in range(18)]
+    else:  # one long sequence and short ones: rows with enough partials for the merge of long rows
+        seg, paths = [16 * 512 + 77] + [40 + 300 * i for i in range(9)], [[i] for i in range(10)]
+    w = make_forest_workload("nan", seg, paths, g, num_q_heads=hq, num_kv_heads=hkv, head_dim=d, kv_dtype=FP8, poison_unused=True)
+    scales = _random_scales(g, w.kv_cache, _used_blocks(w.block_table, w.seq_lens), powers=True)
+    clean, cache = w.kv_cache, w.kv_cache.clone()
+    bad = torch.zeros(w.num_seqs, hkv, dtype=torch.bool)
+    for s in range(0, w.num_seqs, 2):
+        at, head = int(torch.randint(0, int(w.seq_lens[s]), (1,), generator=g)), s // 2 % hkv
+        blk = int(w.block_table[s, at // 16])
+        cache.view(torch.uint8)[0, blk, head].view(d // 16, 16, 16)[3, at % 16, 5] = 0x7F
+        for o in range(w.num_seqs):
+            where = (w.block_table[o, : (int(w.seq_lens[o]) + 15) // 16] == blk).nonzero()
+            bad[o, head] |= bool(len(where)) and int(where[0]) * 16 + at % 16 < int(w.seq_lens[o])
+    out, lse = _attend(emu, w.q, cache, scales, w.block_table, w.seq_lens, w.scale, hq, hkv, d, chunk, rows, workgroups=8 if hkv > 1 else 2)
+    bad = bad.repeat_interleave(4, dim=1)
+    assert torch.equal(lse.isnan(), bad) and torch.equal(out.isnan(), bad[..., None].expand_as(out))
+    ref, ref_lse, _, _ = oracle.attention(w.q, clean, scales, w.block_table, range(w.num_seqs), w.seq_lens.tolist(), w.scale)
+    keep = torch.where(bad[..., None], ref.bfloat16(), out), torch.where(bad, ref_lse.float(), lse)
+    _check_attention(*keep, w.q, clean, scales, w.block_table, range(w.num_seqs), w.seq_lens.tolist(), w.scale, "nan keys")
+
+
 @pytest.mark.parametrize("d,hkv,t", [(64, 3, 70), (128, 1, 300), (256, 2, 5)])
 def test_append_and_gather(emu, order, d, hkv, t):  # noqa: F811
     g = torch.Generator().manual_seed(t)
