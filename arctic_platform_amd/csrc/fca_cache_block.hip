@@ -22,6 +22,7 @@
 namespace fca {
 
 typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+typedef int64_t i64x2 __attribute__((ext_vector_type(2)));
 
 __device__ inline float bf16_float(unsigned short x) { return __uint_as_float((unsigned)x << 16); }
 __device__ inline float bf16_low(unsigned w) { return __uint_as_float(w << 16); }
@@ -104,6 +105,67 @@ __device__ inline ScaleStep step_scale(float* at, float was, unsigned lane_amax,
   return s;
 }
 
+// A block that gets few tokens is not read unless its scale grows (then behind the reduction): its
+// other codes stay where they are.  With more of them the old codes are fetched along with the rows.
+constexpr int kFewTokens = 4;
+
+// `win`: the call's token at every offset of the block, -1 = none.
+template <int D>
+__device__ inline void append_k_tile(const BlockCacheParams& p, const int* win, int64_t blk, int h, int lane) {
+  constexpr int U = D / 64;  // 16-byte units of the tile per lane
+  const int tok = lane & 15;
+  const int t = win[tok];
+  float* at = p.scales + (blk * p.num_kv_heads + h) * 2;
+  const float was = *at;  // (every lane has it before the reduction, lane 0 writes behind it)
+  char* tile = static_cast<char*>(p.k_cache) + blk * p.cache_block_stride + h * p.cache_head_stride;
+  const unsigned short* row = static_cast<const unsigned short*>(p.key) + (int64_t)t * p.token_stride + (int64_t)h * p.head_stride;
+  const bool few = __popcll(__ballot(t >= 0)) <= 4 * kFewTokens;
+  unsigned in[U * 8];
+  union Codes {
+    int4 raw;
+    unsigned w[4];
+  } out[U];
+#pragma unroll
+  for (int i = 0; i < U; ++i) {
+    const int c = (lane >> 4) + 4 * i;
+    int4 x0 = make_int4(0, 0, 0, 0), x1 = x0;
+    if (t >= 0) {
+      x0 = *reinterpret_cast<const int4*>(row + 16 * c);
+      x1 = *reinterpret_cast<const int4*>(row + 16 * c + 8);
+    } else if (!few) {
+      out[i].raw = *reinterpret_cast<const int4*>(tile + (c * kBlock + tok) * 16);
+    }
+    in[8 * i] = x0.x, in[8 * i + 1] = x0.y, in[8 * i + 2] = x0.z, in[8 * i + 3] = x0.w;
+    in[8 * i + 4] = x1.x, in[8 * i + 5] = x1.y, in[8 * i + 6] = x1.z, in[8 * i + 7] = x1.w;
+  }
+  bool special;
+  const unsigned amax = lane_max(in, special);
+  const ScaleStep s = step_scale(at, was, amax, special, win[0] >= 0, lane);
+  if (t < 0) {
+    if (!s.grown) return;
+    if (few) {
+#pragma unroll
+      for (int i = 0; i < U; ++i) out[i].raw = *reinterpret_cast<const int4*>(tile + (((lane >> 4) + 4 * i) * kBlock + tok) * 16);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < U; ++i) {
+    const int c = (lane >> 4) + 4 * i;
+    if (t >= 0) {
+#pragma unroll
+      for (int d = 0; d < 4; ++d) {
+        const unsigned lo = in[8 * i + 2 * d], hi = in[8 * i + 2 * d + 1];
+        const float x0 = bf16_low(lo) * s.inv, x1 = bf16_high(lo) * s.inv, x2 = bf16_low(hi) * s.inv, x3 = bf16_high(hi) * s.inv;
+        out[i].w[d] = s.special ? e4m3_codes(x0, x1, x2, x3) : e4m3_codes_of_small(x0, x1, x2, x3);
+      }
+    } else {
+#pragma unroll
+      for (int d = 0; d < 4; ++d) out[i].w[d] = rescaled_codes(out[i].w[d], s.ratio);
+    }
+    *reinterpret_cast<int4*>(tile + (c * kBlock + tok) * 16) = out[i].raw;
+  }
+}
+
 // CH adjacent bf16 numbers (an element access of 2, 4 or 8 bytes) as dwords.
 template <int CH>
 __device__ inline void load_channels(const unsigned short* from, unsigned (&w)[(CH + 1) / 2]) {
@@ -117,75 +179,55 @@ __device__ inline void load_channels(const unsigned short* from, unsigned (&w)[(
   }
 }
 
-// K and V of one block and KV head; all loads of both are in flight together.  `win`: the call's token at
-// every offset of the block, -1 = none.
 template <int D>
-__device__ inline void append_tiles(const BlockCacheParams& p, const int* win, int64_t blk, int h, int lane) {
-  constexpr int U = D / 64;            // K: 16-byte units of the tile per lane
-  constexpr int CH = D / 64;           // V: adjacent channels per lane
-  constexpr int W = (CH + 1) / 2;      // ... as dwords
+__device__ inline void append_v_tile(const BlockCacheParams& p, const int* win, int64_t blk, int h, int lane) {
+  constexpr int CH = D / 64;  // adjacent channels per lane
+  constexpr int W = (CH + 1) / 2;
+  float* at = p.scales + (blk * p.num_kv_heads + h) * 2 + 1;
+  const float was = *at;
+  char* tile = static_cast<char*>(p.v_cache) + blk * p.cache_block_stride + h * p.cache_head_stride + lane * CH * kBlock;
+  const unsigned short* rows = static_cast<const unsigned short*>(p.value) + (int64_t)h * p.head_stride + lane * CH;
+  const int mine = win[lane & 15];
+  const unsigned live = (unsigned)(__ballot(mine >= 0) & 0xffff);
   union Codes {
     int4 raw;
     unsigned w[4];
-  };
-  const int tok = lane & 15;
-  const int mine = win[tok];
-  const unsigned live = (unsigned)(__ballot(mine >= 0) & 0xffff);
-  const bool begins = live & 1;
-  float* at = p.scales + (blk * p.num_kv_heads + h) * 2;
-  const float k_was = at[0], v_was = at[1];  // (every lane has them before the reductions, lane 0 writes behind those)
-  const int64_t tile_at = blk * p.cache_block_stride + h * p.cache_head_stride;
-  char* k_tile = static_cast<char*>(p.k_cache) + tile_at;
-  char* v_tile = static_cast<char*>(p.v_cache) + tile_at + lane * CH * kBlock;
-  const unsigned short* k_row = static_cast<const unsigned short*>(p.key) + (int64_t)mine * p.token_stride + (int64_t)h * p.head_stride;
-  const unsigned short* v_rows = static_cast<const unsigned short*>(p.value) + (int64_t)h * p.head_stride + lane * CH;
-
-  unsigned k_in[U * 8];
-  Codes k_out[U], v_out[CH];
+  } old[CH];
+  const bool few = __popc(live) <= kFewTokens;
+  if (live != 0xffff && !few) {
 #pragma unroll
-  for (int i = 0; i < U; ++i) {
-    const int c = (lane >> 4) + 4 * i;
-    int4 x0 = make_int4(0, 0, 0, 0), x1 = x0;
-    if (mine >= 0) {
-      x0 = *reinterpret_cast<const int4*>(k_row + 16 * c);
-      x1 = *reinterpret_cast<const int4*>(k_row + 16 * c + 8);
-    } else {
-      k_out[i].raw = *reinterpret_cast<const int4*>(k_tile + (c * kBlock + tok) * 16);
-    }
-    k_in[8 * i] = x0.x, k_in[8 * i + 1] = x0.y, k_in[8 * i + 2] = x0.z, k_in[8 * i + 3] = x0.w;
-    k_in[8 * i + 4] = x1.x, k_in[8 * i + 5] = x1.y, k_in[8 * i + 6] = x1.z, k_in[8 * i + 7] = x1.w;
+    for (int ch = 0; ch < CH; ++ch) old[ch].raw = *reinterpret_cast<const int4*>(tile + ch * kBlock);
+  } else {
+#pragma unroll
+    for (int ch = 0; ch < CH; ++ch) old[ch].raw = make_int4(0, 0, 0, 0);
   }
-#pragma unroll
-  for (int ch = 0; ch < CH; ++ch)
-    v_out[ch].raw = live != 0xffff ? *reinterpret_cast<const int4*>(v_tile + ch * kBlock) : make_int4(0, 0, 0, 0);
-  unsigned v_in[kBlock * W];
+  unsigned in[kBlock * W];
 #pragma unroll
   for (int k = 0; k < kBlock; ++k) {
     const int t = __builtin_amdgcn_readlane(mine, k);
     unsigned w[W] = {};
-    if (t >= 0) load_channels<CH>(v_rows + (int64_t)t * p.token_stride, w);
+    if (t >= 0) load_channels<CH>(rows + (int64_t)t * p.token_stride, w);
 #pragma unroll
-    for (int i = 0; i < W; ++i) v_in[k * W + i] = w[i];
+    for (int i = 0; i < W; ++i) in[k * W + i] = w[i];
   }
-
-  bool k_special, v_special;
-  const unsigned k_amax = lane_max(k_in, k_special), v_amax = lane_max(v_in, v_special);
-  const ScaleStep ks = step_scale(at, k_was, k_amax, k_special, begins, lane);
-  const ScaleStep vs = step_scale(at + 1, v_was, v_amax, v_special, begins, lane);
-
-  if (mine >= 0 || ks.grown) {
+  bool special;
+  const unsigned amax = lane_max(in, special);
+  const ScaleStep s = step_scale(at, was, amax, special, live & 1, lane);
+  if (few && !s.grown) {
 #pragma unroll
-    for (int i = 0; i < U; ++i) {
-      const int c = (lane >> 4) + 4 * i;
+    for (int k = 0; k < kBlock; ++k) {
+      if (!(live >> k & 1)) continue;
 #pragma unroll
-      for (int d = 0; d < 4; ++d) {
-        const unsigned lo = k_in[8 * i + 2 * d], hi = k_in[8 * i + 2 * d + 1];
-        const float x0 = bf16_low(lo) * ks.inv, x1 = bf16_high(lo) * ks.inv, x2 = bf16_low(hi) * ks.inv, x3 = bf16_high(hi) * ks.inv;
-        if (mine < 0) k_out[i].w[d] = rescaled_codes(k_out[i].w[d], ks.ratio);
-        else k_out[i].w[d] = ks.special ? e4m3_codes(x0, x1, x2, x3) : e4m3_codes_of_small(x0, x1, x2, x3);
+      for (int ch = 0; ch < CH; ++ch) {
+        const unsigned w = in[k * W + ch / 2];
+        tile[ch * kBlock + k] = (char)e4m3_code((ch & 1 ? bf16_high(w) : bf16_low(w)) * s.inv);
       }
-      *reinterpret_cast<int4*>(k_tile + (c * kBlock + tok) * 16) = k_out[i].raw;
     }
+    return;
+  }
+  if (few) {
+#pragma unroll
+    for (int ch = 0; ch < CH; ++ch) old[ch].raw = *reinterpret_cast<const int4*>(tile + ch * kBlock);
   }
 #pragma unroll
   for (int ch = 0; ch < CH; ++ch) {
@@ -194,17 +236,17 @@ __device__ inline void append_tiles(const BlockCacheParams& p, const int* win, i
       float x[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const unsigned w = v_in[(4 * d + e) * W + ch / 2];
-        x[e] = (ch & 1 ? bf16_high(w) : bf16_low(w)) * vs.inv;
+        const unsigned w = in[(4 * d + e) * W + ch / 2];
+        x[e] = (ch & 1 ? bf16_high(w) : bf16_low(w)) * s.inv;
       }
-      const unsigned q = vs.special ? e4m3_codes(x[0], x[1], x[2], x[3]) : e4m3_codes_of_small(x[0], x[1], x[2], x[3]);
+      const unsigned q = s.special ? e4m3_codes(x[0], x[1], x[2], x[3]) : e4m3_codes_of_small(x[0], x[1], x[2], x[3]);
       // bytes of the call's tokens (the same in every lane)
       const unsigned four = (live >> (4 * d)) & 15;
       const unsigned fresh = ((four & 1) | (four & 2) << 7 | (four & 4) << 14 | (four & 8) << 21) * 0xffu;
-      const unsigned kept = vs.grown ? rescaled_codes(v_out[ch].w[d], vs.ratio) : v_out[ch].w[d];
-      v_out[ch].w[d] = (q & fresh) | (kept & ~fresh);
+      const unsigned kept = s.grown ? rescaled_codes(old[ch].w[d], s.ratio) : old[ch].w[d];
+      old[ch].w[d] = (q & fresh) | (kept & ~fresh);
     }
-    *reinterpret_cast<int4*>(v_tile + ch * kBlock) = v_out[ch].raw;
+    *reinterpret_cast<int4*>(tile + ch * kBlock) = old[ch].raw;
   }
 }
 
@@ -213,13 +255,14 @@ __device__ inline void append_tiles(const BlockCacheParams& p, const int* win, i
 // tokens belong to them, it finds by looking at all slots of the call: they are few next to the rows
 // (8 bytes a token against 4 D Hkv), come out of the L2, and nothing has to be known about their order.
 constexpr int kMaxWindow = 64;
+constexpr int kAppendThreads = 512;  // at most
 template <int D>
-__global__ __launch_bounds__(256) void fca_append_block_kernel(BlockCacheParams p, int window, int heads, int head_groups) {
+__global__ __launch_bounds__(kAppendThreads) void fca_append_block_kernel(BlockCacheParams p, int window, int heads, int head_groups) {
   __shared__ int cand[kMaxWindow];         // blocks of the window's tokens, each once
   __shared__ int win[kMaxWindow][kBlock];  // the call's last token at every offset of theirs, -1 = none
   __shared__ int foreign[kMaxWindow];      // the block has a token in front of the window
   __shared__ int num_cand;
-  const int tid = threadIdx.x;
+  const int tid = threadIdx.x, threads = blockDim.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int w = blockIdx.x / head_groups, h0 = (blockIdx.x - w * head_groups) * heads;
   const int t0 = w * window;
@@ -239,38 +282,54 @@ __global__ __launch_bounds__(256) void fca_append_block_kernel(BlockCacheParams 
     if (leads) cand[__popcll(all & ((1ull << lane) - 1))] = blk;
     if (lane == 0) num_cand = __popcll(all);
   }
-  for (int j = tid; j < window * kBlock; j += 256) (&win[0][0])[j] = -1;
+  for (int j = tid; j < window * kBlock; j += threads) (&win[0][0])[j] = -1;
   if (tid < kMaxWindow) foreign[tid] = 0;
   __syncthreads();
   const int n = num_cand;
   if (n == 0) return;
-  // (kScan slots per thread and trip, whose loads are in flight together)
-  constexpr int kScan = 16;
-  for (int base = 0; base < p.num_tokens; base += 256 * kScan) {
-    int64_t slots[kScan];
+  // (pairs of adjacent slots; kScan loads of a thread in flight together.  Workgroups begin at different
+  // places, or all would ask the same channel of the cache for the same line at the same time.)
+  constexpr int kScan = 2;
+  const int trip = 2 * kScan * threads;
+  const int trips = (p.num_tokens + trip - 1) / trip;
+  for (int i = 0; i < trips; ++i) {
+    const int base = (int)((i + blockIdx.x) % trips) * trip;
+    i64x2 slots[kScan];
 #pragma unroll
     for (int k = 0; k < kScan; ++k) {
-      const int t = base + 256 * k + tid;
-      slots[k] = t < p.num_tokens ? p.slot_mapping[t] : -1;
+      const int t = base + 2 * (k * threads + tid);
+      slots[k] = i64x2{-1, -1};
+      if (t + 1 < p.num_tokens)
+        __builtin_memcpy(&slots[k], p.slot_mapping + t, 16);
+      else if (t < p.num_tokens)
+        slots[k][0] = p.slot_mapping[t];
     }
+    for (int c = 0; c < n; ++c) {
+      const int64_t first = (int64_t)cand[c] * kBlock;
 #pragma unroll
-    for (int k = 0; k < kScan; ++k) {
-      if (base + 256 * k >= p.num_tokens) break;
-      const int blk = slots[k] >= 0 && slots[k] < end ? (int)(slots[k] / kBlock) : -1;
-      const int t = base + 256 * k + tid;
-      for (int c = 0; c < n; ++c) {
-        if (blk != cand[c]) continue;
-        if (t < t0) foreign[c] = 1;
-        else atomicMax(&win[c][(int)slots[k] & (kBlock - 1)], t);
+      for (int k = 0; k < kScan; ++k) {
+        const int t = base + 2 * (k * threads + tid);
+        const uint64_t x = slots[k][0] - first, y = slots[k][1] - first;
+        if (x < kBlock) {
+          if (t < t0) foreign[c] = 1;
+          else atomicMax(&win[c][x], t);
+        }
+        if (y < kBlock) {
+          if (t + 1 < t0) foreign[c] = 1;
+          else atomicMax(&win[c][y], t + 1);
+        }
       }
     }
   }
   __syncthreads();
-  const int tasks = n * heads;
-  for (int j = wave; j < tasks; j += 4) {
-    const int c = j / heads, h = h0 + j - c * heads;
+  const int tasks = n * heads * 2;
+  for (int j = wave; j < tasks; j += threads / 64) {
+    const int c = j / (2 * heads), rest = j - c * 2 * heads, h = h0 + (rest >> 1);
     if (foreign[c] || h >= p.num_kv_heads) continue;
-    append_tiles<D>(p, win[c], cand[c], h, lane);
+    if (rest & 1)
+      append_v_tile<D>(p, win[c], cand[c], h, lane);
+    else
+      append_k_tile<D>(p, win[c], cand[c], h, lane);
   }
 }
 
@@ -381,22 +440,26 @@ __global__ __launch_bounds__(256) void fca_gather_block_kernel(BlockCacheParams 
 
 hipError_t launch_append_block(const BlockCacheParams& p, hipStream_t stream) {
   if (p.num_tokens == 0) return hipSuccess;
-  // Windows: at most 512 of them up to their largest size (few workgroups look at all the slots);
-  // KV heads: as many groups as bring the launch to about 1024 workgroups.
+  // Windows: at most 512 of them up to their largest size; KV heads: as many groups as bring the launch
+  // to 512 workgroups; waves: one for each two tiles of a workgroup, 4 to 8.  Few large workgroups
+  // look at all the slots: 8191 tokens of 8 heads take 17 us, with 1024 workgroups of 4 waves 21, with
+  // twice as many windows 26; 8 tokens take 4.4 (an empty launch: 2.5), 512 tokens of 512 blocks 9.2.
   int window = 1;
   while (window < kMaxWindow && (p.num_tokens + window - 1) / window > 512) window *= 2;
   const int windows = (p.num_tokens + window - 1) / window;
-  int groups = (1024 + windows - 1) / windows;
+  int groups = (512 + windows - 1) / windows;
   if (groups > p.num_kv_heads) groups = p.num_kv_heads;
   const int heads = (p.num_kv_heads + groups - 1) / groups;
   groups = (p.num_kv_heads + heads - 1) / heads;
   const dim3 grid(windows * groups);
+  int threads = 64 * heads * (window > 1 ? 2 : 1);
+  threads = threads < 256 ? 256 : threads > kAppendThreads ? kAppendThreads : threads;
   if (p.head_dim == 64)
-    hipLaunchKernelGGL(fca_append_block_kernel<64>, grid, dim3(256), 0, stream, p, window, heads, groups);
+    hipLaunchKernelGGL(fca_append_block_kernel<64>, grid, dim3(threads), 0, stream, p, window, heads, groups);
   else if (p.head_dim == 128)
-    hipLaunchKernelGGL(fca_append_block_kernel<128>, grid, dim3(256), 0, stream, p, window, heads, groups);
+    hipLaunchKernelGGL(fca_append_block_kernel<128>, grid, dim3(threads), 0, stream, p, window, heads, groups);
   else
-    hipLaunchKernelGGL(fca_append_block_kernel<256>, grid, dim3(256), 0, stream, p, window, heads, groups);
+    hipLaunchKernelGGL(fca_append_block_kernel<256>, grid, dim3(threads), 0, stream, p, window, heads, groups);
   return hipGetLastError();
 }
 
