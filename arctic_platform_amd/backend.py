@@ -35,7 +35,7 @@ import torch
 from .cache import append_kv, gather_kv
 from .config import ModelConfig, validate_fca_support
 from .forest import ForestMetadata, build_forest_metadata, rows_from_query_runs
-from .kv_layout import BLOCK_SIZE, kv_cache_shape
+from .kv_layout import BLOCK_SIZE, block_scales_shape, kv_cache_shape
 from .ops import forest_cascade_decode
 from .split_attention import SplitLayout, split_attention_forward
 
@@ -115,6 +115,12 @@ class ForestCascadeAttentionBackend:
     @staticmethod
     def get_kv_cache_shape(num_blocks: int, block_size: int, num_kv_heads: int, head_size: int):
         return kv_cache_shape(num_blocks, block_size, num_kv_heads, head_size)
+
+    @staticmethod
+    def get_kv_block_scales_shape(num_blocks: int, num_kv_heads: int):
+        """Shape of the fp32 table that a layer keeps next to its cache (``layer.kv_block_scales``)
+        when the job runs with ``kv_cache_dtype="fp8_block"``."""
+        return block_scales_shape(num_blocks, num_kv_heads)
 
 
 class ForestCascadeMetadataBuilder:
@@ -351,11 +357,19 @@ class ForestCascadeAttentionImpl:
     def forward(self, layer, query, key, value, kv_cache, attn_metadata: ForestCascadeMetadata, output=None):
         """query ``[T, Hq*D]`` or ``[T, Hq, D]``; key/value ``[T, Hkv*D]`` / ``[T, Hkv, D]`` or
         None when the cache already holds the step's tokens; returns ``output`` shaped like
-        ``query``.  Per-KV-head fp8 scales are read from ``layer.k_scale`` / ``layer.v_scale``."""
+        ``query``.  Per-KV-head fp8 scales are read from ``layer.k_scale`` / ``layer.v_scale``.
+        With ``kv_cache_dtype="fp8_block"`` the scales are those of ``layer.kv_block_scales``, written
+        here along with the cache, and per-head scales that a layer may also have are not used."""
         t = attn_metadata.num_decode_tokens
         q = query[:t].view(t, self.num_heads, self.head_size)
-        k_scale = getattr(layer, "k_scale", None)
-        v_scale = getattr(layer, "v_scale", None)
+        k_scale = v_scale = block_scales = None
+        if self.kv_cache_dtype == "fp8_block":
+            block_scales = getattr(layer, "kv_block_scales", None)
+            if block_scales is None:
+                raise ValueError("kv_cache_dtype 'fp8_block' needs layer.kv_block_scales (get_kv_block_scales_shape)")
+        else:
+            k_scale = getattr(layer, "k_scale", None)
+            v_scale = getattr(layer, "v_scale", None)
         if key is not None:
             append_kv(
                 key[:t].view(t, self.num_kv_heads, self.head_size),
@@ -364,6 +378,7 @@ class ForestCascadeAttentionImpl:
                 attn_metadata.slot_mapping,
                 k_scale,
                 v_scale,
+                block_scales=block_scales,
             )
         if output is None:
             output = torch.empty_like(query)
@@ -372,7 +387,9 @@ class ForestCascadeAttentionImpl:
                 raise ValueError("a step with fresh prompts needs the step's key and value")
             f = attn_metadata.fresh_start
             if attn_metadata.context_slots is not None:  # context and chunk alike, from the cache just filled
-                k_rows, v_rows = gather_kv(kv_cache, attn_metadata.context_slots, self.head_size, k_scale, v_scale)
+                k_rows, v_rows = gather_kv(
+                    kv_cache, attn_metadata.context_slots, self.head_size, k_scale, v_scale, block_scales=block_scales
+                )
             else:
                 k_rows = key[f:t].view(t - f, self.num_kv_heads, self.head_size)
                 v_rows = value[f:t].view(t - f, self.num_kv_heads, self.head_size)
@@ -385,6 +402,6 @@ class ForestCascadeAttentionImpl:
             t, q = f, q[:f]
         forest_cascade_decode(
             q, kv_cache, attn_metadata.forest, self.scale, k_scale, v_scale,
-            out=output[:t].view(t, self.num_heads, self.head_size), return_lse=False,
+            out=output[:t].view(t, self.num_heads, self.head_size), return_lse=False, block_scales=block_scales,
         )
         return output
