@@ -21,25 +21,30 @@
 
 namespace fca {
 
-// Direct-to-LDS loads: every lane's 16 bytes land at lds_slot + lane * 16.  Written as assembly so
-// that the compiler's wait insertion does not know of them (it would drain them before every LDS
-// read); loads it does not know of only make its own waits more conservative.  M0 is restored.
+// Direct-to-LDS loads: a wave copies `PIECES` KB of a block to LDS as they lie.  An instruction moves 16
+// bytes per lane to M0 + 16 * lane, and its immediate offset counts on both sides.  Written as assembly so
+// that the compiler's wait insertion does not know of the loads (it would drain them before every LDS
+// read); loads it does not know of only make its own waits more conservative.
 __device__ inline unsigned lds_address(const void* p) {
   return __builtin_amdgcn_readfirstlane((unsigned)(size_t)((__attribute__((address_space(3))) void*)(p)));
 }
-__device__ inline void load_to_lds16(const void* src, unsigned lds_slot) {
-  unsigned saved;
-  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %1, off\n\ts_mov_b32 m0, %0"
-               : "=&s"(saved)
-               : "v"(src), "s"(lds_slot)
-               : "memory");
-}
-__device__ inline void stream_to_lds16(const void* src, unsigned lds_slot) {
-  unsigned saved;
-  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %1, off nt\n\ts_mov_b32 m0, %0"
-               : "=&s"(saved)
-               : "v"(src), "s"(lds_slot)
-               : "memory");
+template <int PIECES, bool STREAM>
+__device__ inline void block_to_lds(const char* block, int lane_off, unsigned lds) {
+  static_assert(PIECES == 1 || PIECES == 2 || PIECES == 4, "");
+#define FCA_TO_LDS(MORE, NT) \
+  asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" NT MORE : : "v"(lane_off), "s"(block), "s"(lds) : "memory", "m0")
+#define FCA_PIECE(OFF, NT) "\n\tglobal_load_lds_dwordx4 %0, %1 offset:" OFF NT
+  if constexpr (STREAM) {
+    if constexpr (PIECES == 1) FCA_TO_LDS("", " nt");
+    if constexpr (PIECES == 2) FCA_TO_LDS(FCA_PIECE("1024", " nt"), " nt");
+    if constexpr (PIECES == 4) FCA_TO_LDS(FCA_PIECE("1024", " nt") FCA_PIECE("2048", " nt") FCA_PIECE("3072", " nt"), " nt");
+  } else {
+    if constexpr (PIECES == 1) FCA_TO_LDS("", "");
+    if constexpr (PIECES == 2) FCA_TO_LDS(FCA_PIECE("1024", ""), "");
+    if constexpr (PIECES == 4) FCA_TO_LDS(FCA_PIECE("1024", "") FCA_PIECE("2048", "") FCA_PIECE("3072", ""), "");
+  }
+#undef FCA_PIECE
+#undef FCA_TO_LDS
 }
 // s_waitcnt that constrains only the vector-memory counter (gfx9 encoding)
 #define FCA_WAIT_VMCNT(n) __builtin_amdgcn_s_waitcnt(0x0f70 | ((n) & 15) | (((n) >> 4) << 14))
@@ -51,7 +56,8 @@ struct WideTuning {
   static constexpr int kWorkgroups = kChannels ? 3 : 4;  // per CU (160 KB of LDS)
   static constexpr int kSlots = kChannels ? 3 : 4;
   static constexpr int kAhead = kSlots - 1;
-  static constexpr int kSlotPieces = D / 16;             // 1 KB pieces of a tile: K's D / 32, then V's D / 32
+  static constexpr int kBlockPieces = D / 64;            // 1 KB pieces of a block's K or V
+  static constexpr int kSlotBytes = 4 * D * kBlock;      // a tile: K of its two blocks, V of its two blocks
   static constexpr int kStripRows = 8;                   // rows a wave writes out at a time
   static constexpr bool kEarlyQ = !kChannels;            // the next item's query rows are fetched an item ahead
 };
@@ -64,7 +70,7 @@ __global__ __launch_bounds__(128, 2) void fca_attend_block_wide_kernel(AttendPar
   constexpr int NK = D / 32, NI = D / 32; // pieces of K; pieces a wave requests per tile
   constexpr int kAhead = Tune::kAhead;
 
-  __shared__ __attribute__((aligned(16))) char ring[Tune::kSlots][Tune::kSlotPieces * 1024];
+  __shared__ __attribute__((aligned(16))) char ring[Tune::kSlots][Tune::kSlotBytes];
   __shared__ __attribute__((aligned(16))) char strips[2][Tune::kStripRows * strip_row_bytes<Tune::kWaveD>()];
   __shared__ float row_amax[2][32];
 
@@ -94,8 +100,9 @@ __global__ __launch_bounds__(128, 2) void fca_attend_block_wide_kernel(AttendPar
   // MFMA row m carries the token whose index has bits 2 and 3 of m swapped: the score accumulator then
   // holds, per lane half, tokens 8h..8h+7 of each block in register order.
   const int tok_of_m = (m & 3) | ((m & 4) << 1) | ((m & 8) >> 1);
-  // where this lane's bytes of a tile are: wave 0 requests K, wave 1 V
-  const int lane_off = wave == 0 ? h * 256 + tok_of_m * 16 : (h * 32 + m) * 16;
+  const int k_off = (m >> 4) * D * kBlock + h * 256 + tok_of_m * 16;  // of a lane's codes in a tile
+  const int v_off = 2 * D * kBlock + (channel0 + m) * kBlock + h * 8;
+  // wave 0 requests K, wave 1 V
   const char* plane = wave == 0 ? p.k_cache : p.v_cache;
 
   // Every ticket is dealt in advance: back and forth over the size-ordered list.
@@ -145,25 +152,10 @@ __global__ __launch_bounds__(128, 2) void fca_attend_block_wide_kernel(AttendPar
   auto request = [&](const Item& x, int blk_ids, int ti) {
     const int b0 = __builtin_amdgcn_readlane(blk_ids, 2 * ti);
     const int b1 = __builtin_amdgcn_readlane(blk_ids, min(2 * ti + 1, blocks_of(x) - 1));
-    const char* base = plane + (int64_t)x.kvh * p.kv_head_bytes + lane_off;
-    const unsigned to = ring_lds + req_slot * (Tune::kSlotPieces * 1024) + wave * (NI * 1024);
-    auto load = [&](const char* src, unsigned slot) {
-      if constexpr (STREAM) stream_to_lds16(src, slot);
-      else load_to_lds16(src, slot);
-    };
-    if (wave == 0) {
-      const char* src = base + (int64_t)((m & 16) ? b1 : b0) * p.kv_block_bytes;
-#pragma unroll
-      for (int i = 0; i < NI; ++i) load(src + i * 512, to + i * 1024);
-    } else {
-      const char* src0 = base + (int64_t)b0 * p.kv_block_bytes;
-      const char* src1 = base + (int64_t)b1 * p.kv_block_bytes;
-#pragma unroll
-      for (int i = 0; i < NI / 2; ++i) {
-        load(src0 + i * 1024, to + (2 * i) * 1024);
-        load(src1 + i * 1024, to + (2 * i + 1) * 1024);
-      }
-    }
+    const char* base = plane + (int64_t)x.kvh * p.kv_head_bytes;
+    const unsigned to = ring_lds + req_slot * Tune::kSlotBytes + wave * (2 * D * kBlock);
+    block_to_lds<Tune::kBlockPieces, STREAM>(base + (int64_t)b0 * p.kv_block_bytes, lane * 16, to);
+    block_to_lds<Tune::kBlockPieces, STREAM>(base + (int64_t)b1 * p.kv_block_bytes, lane * 16, to + D * kBlock);
     req_slot = req_slot + 1 == Tune::kSlots ? 0 : req_slot + 1;
   };
 
@@ -214,7 +206,6 @@ __global__ __launch_bounds__(128, 2) void fca_attend_block_wide_kernel(AttendPar
 
     auto compute_tile = [&](int ti, auto ragged) {
       constexpr bool RAGGED = decltype(ragged)::value;
-      const i32x4* tile = reinterpret_cast<const i32x4*>(&ring[slot][0]) + lane;  // piece j of this lane: tile[64 * j]
       const int tok0 = ti * kTile;
       float ks[2], vs[2];
 #pragma unroll
@@ -228,7 +219,7 @@ __global__ __launch_bounds__(128, 2) void fca_attend_block_wide_kernel(AttendPar
       i32x4 kw[NK];
       i32x2 vw[2][NDB];
 #pragma unroll
-      for (int i = 0; i < NK; ++i) kw[i] = tile[64 * i];
+      for (int i = 0; i < NK; ++i) kw[i] = *reinterpret_cast<const i32x4*>(&ring[slot][0] + k_off + 512 * i);
       __builtin_amdgcn_sched_barrier(0);
       f32x16 sr;
 #pragma unroll
@@ -238,13 +229,12 @@ __global__ __launch_bounds__(128, 2) void fca_attend_block_wide_kernel(AttendPar
         sr = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fp8x8_to_bf16(kw[i][0], kw[i][1]), qreg[2 * i], sr, 0, 0, 0);
         sr = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fp8x8_to_bf16(kw[i][2], kw[i][3]), qreg[2 * i + 1], sr, 0, 0, 0);
       }
-      // codes of tokens 8h..8h+7 of channel 32 * db + m: its 16 tokens lie together in a piece of 64 channels
-      const char* values = &ring[slot][0] + (NK + 2 * (channel0 / 64)) * 1024 + m * 16 + h * 8;
+      // codes of tokens 8h..8h+7 of channel 32 * db + m
 #pragma unroll
       for (int db = 0; db < NDB; ++db)
 #pragma unroll
         for (int blk = 0; blk < 2; ++blk)
-          vw[blk][db] = *reinterpret_cast<const i32x2*>(values + (2 * (db >> 1) + blk) * 1024 + (db & 1) * 512);
+          vw[blk][db] = *reinterpret_cast<const i32x2*>(&ring[slot][0] + v_off + (blk * D + 32 * db) * kBlock);
       __builtin_amdgcn_sched_barrier(0);
       // register r holds token 16 * (r / 8) + 8 * h + r % 8 of the tile, for this lane's query row
       if constexpr (RAGGED) {

@@ -166,3 +166,27 @@ def test_a_launch_requests_every_block_about_once(emu):  # noqa: F811
         asked = emu.emu_take_streamed_bytes() / 2
         partials = 4 * 12 * hq * (2 * d + 8) * 3  # (the merge reads its partial rows with streaming loads too)
         assert asked - partials <= 1.25 * w.unique_tokens * 2 * hkv * d, (rows, asked, w.unique_tokens * 2 * hkv * d)
+
+
+@pytest.mark.parametrize("d,rows,workgroups", [(128, 64, 1), (64, 64, 2), (256, 32, 1), (256, 32, 3)])
+def test_long_query_runs_shared_by_two_workgroups(emu, order, d, rows, workgroups):  # noqa: F811
+    """Items of 16 to 22 tiles whose last tile shows each row another number of tokens, or none: attended by
+    two workgroups, one of which begins with that tile."""
+    hq, hkv = 4, 1
+    g = torch.Generator().manual_seed(d + workgroups)
+    lens, news = [600, 545, 700, 560], [5, 3, 9, 17]
+    q, cache, scales, table, starts, row_table, row_lens = _query_runs(g, lens, news, hq, hkv, d, 32)
+    clean = cache.clone()
+    at = lens[2] - 2
+    cache.view(torch.uint8)[1, int(table[2, at // 16]), 0].view(d, 16)[d // 2 + 3, at % 16] = 0xFF
+    group = torch.tensor([s * table.shape[1] + (n - 1) // 16 for s, n in zip(row_table, row_lens)], dtype=torch.int32)
+    out, lse = _attend(
+        emu, q, cache, scales, table, torch.tensor(row_lens, dtype=torch.int32), 0.1, hq, hkv, d, 1024, rows,
+        row_table=torch.tensor(row_table, dtype=torch.int32), row_group=group, reread=1, workgroups=workgroups,
+    )
+    last = torch.tensor([s == 2 and n > at for s, n in zip(row_table, row_lens)])
+    bad = torch.zeros(out.shape, dtype=torch.bool)
+    bad[last, :, d // 2 + 3] = True
+    assert int(last.sum()) == 2 and torch.equal(out.isnan(), bad) and not lse.isnan().any()
+    ref = oracle.attention(q, clean, scales, table, row_table, row_lens, 0.1)[0]
+    _check_attention(torch.where(bad, ref.bfloat16(), out), lse, q, clean, scales, table, row_table, row_lens, 0.1, "query runs")
