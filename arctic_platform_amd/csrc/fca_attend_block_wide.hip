@@ -58,7 +58,6 @@ struct WideTuning {
   static constexpr int kAhead = kSlots - 1;
   static constexpr int kBlockPieces = D / 64;            // 1 KB pieces of a block's K or V
   static constexpr int kSlotBytes = 4 * D * kBlock;      // a tile: K of its two blocks, V of its two blocks
-  static constexpr int kStripRows = 8;                   // rows a wave writes out at a time
   static constexpr bool kEarlyQ = !kChannels;            // the next item's query rows are fetched an item ahead
 };
 
@@ -71,7 +70,6 @@ __global__ __launch_bounds__(128, 2) void fca_attend_block_wide_kernel(AttendPar
   constexpr int kAhead = Tune::kAhead;
 
   __shared__ __attribute__((aligned(16))) char ring[Tune::kSlots][Tune::kSlotBytes];
-  __shared__ __attribute__((aligned(16))) char strips[2][Tune::kStripRows * strip_row_bytes<Tune::kWaveD>()];
   __shared__ float row_amax[2][32];
 
   const int32_t* hdr = p.meta + p.off_header;
@@ -87,7 +85,6 @@ __global__ __launch_bounds__(128, 2) void fca_attend_block_wide_kernel(AttendPar
   const int G = p.group, Hkv = p.num_kv_heads;
   const int32_t* meta = p.meta;
   const float2* scales = reinterpret_cast<const float2*>(p.k_scale);
-  char* strip = strips[wave];
   const unsigned ring_lds = lds_address(&ring[0][0]);
 
   // Row `row_tile * 32 + m` of the stacked query tile is (member row / G, head row % G).  Which wave
@@ -339,8 +336,9 @@ __global__ __launch_bounds__(128, 2) void fca_attend_block_wide_kernel(AttendPar
       slot = slot + 1 == Tune::kSlots ? 0 : slot + 1;
     }
 
-    // ---- the item's partial rows: normalised, as halves times one power of two per row, through a
-    // strip of LDS so that they leave in whole pieces
+    // ---- the item's partial rows: normalised, as halves times one power of two per row.  A lane has
+    // every other four channels of its row; after a swap with the lane 32 away it has eight adjacent
+    // ones.  (Through a strip of LDS, so that rows leave whole, it took 3 us an item.)
     {
       const float l = lrow + other_half(lrow);
       const float inv = 1.f / l;
@@ -363,44 +361,24 @@ __global__ __launch_bounds__(128, 2) void fca_attend_block_wide_kernel(AttendPar
         if constexpr (STREAM) store8_coherent(p.partial_lse + 2 * prow, __builtin_bit_cast(uint64_t, ls));
         else *reinterpret_cast<f32x2*>(p.partial_lse + 2 * prow) = ls;
       }
-      constexpr int kRowBytes = strip_row_bytes<Tune::kWaveD>();
-      constexpr int LPR = Tune::kWaveD / 8;  // lanes per row, each with 16 bytes of it
       if (has_rows) {
+        char* dst = static_cast<char*>(p.partial_out) + (max(prow, (int64_t)0) * D + channel0 + 8 * h) * 2;
 #pragma unroll
-        for (int part = 0; part < 32 / Tune::kStripRows; ++part) {
-          if (m / Tune::kStripRows == part) {
-            char* dst = strip + (m % Tune::kStripRows) * kRowBytes;
-            if (h == 0) *reinterpret_cast<int64_t*>(dst + Tune::kWaveD * 2) = prow;
+        for (int db = 0; db < NDB; ++db)
 #pragma unroll
-            for (int db = 0; db < NDB; ++db)
+          for (int q = 0; q < 2; ++q) {
+            i32x2 v[2];
 #pragma unroll
-              for (int q4 = 0; q4 < 4; ++q4) {
-                f16x4 v;
+            for (int j = 0; j < 2; ++j) {
+              f16x4 x;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = (_Float16)(acc[db][q4 * 4 + e] * k);
-                *reinterpret_cast<f16x4*>(dst + (db * 32 + q4 * 8 + h * 4) * 2) = v;
-              }
-          }
-          __builtin_amdgcn_wave_barrier();
-          for (int row = lane / LPR; row < Tune::kStripRows; row += 64 / LPR) {
-            const char* src = strip + row * kRowBytes;
-            const int64_t to = *reinterpret_cast<const int64_t*>(src + Tune::kWaveD * 2);
-            const int c = (lane % LPR) * 8;
-            if (to >= 0) {
-              char* dst = static_cast<char*>(p.partial_out) + (to * D + channel0) * 2;
-              const uint64_t lo = *reinterpret_cast<const uint64_t*>(src + c);
-              const uint64_t hi = *reinterpret_cast<const uint64_t*>(src + Tune::kWaveD + c);
-              if constexpr (STREAM) {
-                store8_coherent(dst + c, lo);
-                store8_coherent(dst + Tune::kWaveD + c, hi);
-              } else {
-                *reinterpret_cast<uint64_t*>(dst + c) = lo;
-                *reinterpret_cast<uint64_t*>(dst + Tune::kWaveD + c) = hi;
-              }
+              for (int e = 0; e < 4; ++e) x[e] = (_Float16)(acc[db][8 * q + 4 * j + e] * k);
+              v[j] = __builtin_bit_cast(i32x2, x);
             }
+            const auto s0 = __builtin_amdgcn_permlane32_swap((unsigned)v[0][0], (unsigned)v[1][0], false, false);
+            const auto s1 = __builtin_amdgcn_permlane32_swap((unsigned)v[0][1], (unsigned)v[1][1], false, false);
+            if (prow >= 0) *reinterpret_cast<i32x4*>(dst + (32 * db + 16 * q) * 2) = i32x4{(int)s0[0], (int)s1[0], (int)s0[1], (int)s1[1]};
           }
-          __builtin_amdgcn_wave_barrier();
-        }
       }
     }
 
