@@ -37,7 +37,7 @@ def check_block_scales(block_scales, kv_cache, k_scale, v_scale) -> None:
     if k_scale is not None or v_scale is not None:
         raise ValueError("a cache has either block_scales or per-head k_scale / v_scale")
     want = block_scales_shape(kv_cache.shape[1], kv_cache.shape[2])
-    if block_scales.dtype != torch.float32 or tuple(block_scales.shape) != want or not block_scales.is_contiguous():
+    if block_scales.dtype != torch.float32 or block_scales.shape != want or not block_scales.is_contiguous():
         raise ValueError(f"block_scales must be a contiguous fp32 tensor of shape {list(want)}")
     if block_scales.device != kv_cache.device:
         raise ValueError(f"block_scales are on {block_scales.device}, the cache is on {kv_cache.device}")

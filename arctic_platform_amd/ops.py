@@ -41,19 +41,15 @@ def _tensors(q, kv_cache, meta: ForestMetadata, scale, k_scale, v_scale, f32_ok=
         kv_dtype = _lib.FCA_FP8_E4M3
     else:
         raise TypeError(f"unsupported KV cache dtype {kv_cache.dtype} (bfloat16, float8_e4m3fn, or float32 with a float32 q)")
-    if q.shape != (plan.num_seqs, plan.num_q_heads, plan.head_dim) or q.stride(2) != 1:
-        raise ValueError(f"q must be [{plan.num_seqs}, {plan.num_q_heads}, {plan.head_dim}] with contiguous head_dim")
-    if (
-        kv_cache.dim() != 4
-        or kv_cache.shape[0] != 2
-        or kv_cache.shape[2] != plan.num_kv_heads
-        or kv_cache.shape[3] != BLOCK_SIZE * plan.head_dim
-        or kv_cache.stride(3) != 1
-    ):
+    # (each of these is a call into torch or ctypes and this runs for every layer of every step: once each)
+    d, q_strides, kv_shape, kv_strides = plan.head_dim, q.stride(), kv_cache.shape, kv_cache.stride()
+    if q.shape != (plan.num_seqs, plan.num_q_heads, d) or q_strides[2] != 1:
+        raise ValueError(f"q must be [{plan.num_seqs}, {plan.num_q_heads}, {d}] with contiguous head_dim")
+    if len(kv_shape) != 4 or kv_shape[0] != 2 or kv_shape[2] != plan.num_kv_heads or kv_shape[3] != BLOCK_SIZE * d or kv_strides[3] != 1:
         raise ValueError("kv_cache must be [2, num_blocks, num_kv_heads, 16 * head_dim] (see kv_layout)")
     if not (q.is_cuda and kv_cache.is_cuda):
         raise RuntimeError("forest cascade attention runs on the GPU only; q and kv_cache must be device tensors")
-    for name, sc in (("k_scale", k_scale), ("v_scale", v_scale)):
+    for name, sc in (("k_scale", k_scale), ("v_scale", v_scale)) if k_scale is not None or v_scale is not None else ():
         if sc is not None and (sc.dtype != torch.float32 or sc.shape != (plan.num_kv_heads,) or not sc.is_contiguous()):
             raise ValueError(f"{name} must be a contiguous fp32 tensor of shape [{plan.num_kv_heads}]")
     if block_scales is not None:
@@ -63,25 +59,25 @@ def _tensors(q, kv_cache, meta: ForestMetadata, scale, k_scale, v_scale, f32_ok=
         if not q.device == kv_cache.device == meta.meta.device:
             raise ValueError("q, the cache and the metadata must be on one device")
         kv_dtype, k_scale = _lib.FCA_FP8_E4M3_BLOCK, block_scales
-    esz = kv_cache.element_size()
+    cache, table = kv_cache.data_ptr(), meta.block_table
     return _lib.FcaTensors(
         q.data_ptr(),
-        q.stride(0),
-        q.stride(1),
-        kv_cache.data_ptr(),
-        kv_cache.data_ptr() + kv_cache.stride(0) * esz,
-        kv_cache.stride(1),
-        kv_cache.stride(2),
+        q_strides[0],
+        q_strides[1],
+        cache,
+        cache + kv_strides[0] * kv_cache.element_size(),
+        kv_strides[1],
+        kv_strides[2],
         kv_dtype,
         1 if meta.kv_reread else 0,
-        meta.block_table.data_ptr(),
-        meta.block_table.stride(0),
+        table.data_ptr(),
+        table.stride(0),
         k_scale.data_ptr() if k_scale is not None else None,
         v_scale.data_ptr() if v_scale is not None else None,
         float(scale),
         1 if meta.reproducible else 0,
         int(meta.max_workgroups),
-        int(meta.fp8_tile_buffers) if kv_dtype == _lib.FCA_FP8_E4M3 and plan.head_dim == 128 and plan.rows_per_item == 32 else 0,
+        int(meta.fp8_tile_buffers) if kv_dtype == _lib.FCA_FP8_E4M3 and d == 128 and plan.rows_per_item == 32 else 0,
     )
 
 
@@ -97,15 +93,16 @@ def _check_partials(meta: ForestMetadata, t) -> None:
 
 def _out_args(q, meta, out, out_dtype):
     plan = meta.plan
+    shape = (plan.num_seqs, plan.num_q_heads, plan.head_dim)
     if out is None:
-        out = torch.empty(plan.num_seqs, plan.num_q_heads, plan.head_dim, dtype=out_dtype or torch.bfloat16, device=q.device)
+        out = torch.empty(shape, dtype=out_dtype or torch.bfloat16, device=q.device)
     if out.dtype == torch.bfloat16:
         code = _lib.FCA_BF16
     elif out.dtype == torch.float32:
         code = _lib.FCA_F32
     else:
         raise TypeError("out must be bfloat16 or float32")
-    if out.shape != (plan.num_seqs, plan.num_q_heads, plan.head_dim) or out.stride(2) != 1:
+    if out.shape != shape or out.stride(2) != 1:
         raise ValueError("out must be [num_seqs, num_q_heads, head_dim] with contiguous head_dim")
     return out, code
 
