@@ -306,11 +306,11 @@ __global__ __launch_bounds__(kAppendThreads) void fca_append_block_kernel(BlockC
         slots[k][0] = p.slot_mapping[t];
     }
     for (int c = 0; c < n; ++c) {
-      const int64_t first = (int64_t)cand[c] * kBlock;
+      const uint64_t first = (uint64_t)cand[c] * kBlock;
 #pragma unroll
       for (int k = 0; k < kScan; ++k) {
         const int t = base + 2 * (k * threads + tid);
-        const uint64_t x = slots[k][0] - first, y = slots[k][1] - first;
+        const uint64_t x = (uint64_t)slots[k][0] - first, y = (uint64_t)slots[k][1] - first;  // (a negative slot is far away)
         if (x < kBlock) {
           if (t < t0) foreign[c] = 1;
           else atomicMax(&win[c][x], t);

@@ -176,6 +176,32 @@ def test_append_values_without_a_number(gpu, d):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("t", [1, 2, 37, 700])
+def test_append_of_slots_behind_others(gpu, t):
+    """The slots as a view that begins 8 bytes past a multiple of 16, with slots around it that are not the
+    call's, the extreme ones of the type among them."""
+    from arctic_platform_amd import append_kv
+
+    g = torch.Generator().manual_seed(t)
+    nb, hkv, d = t // 16 + 6, 2, 64
+    cache, scales = _old_state(g, nb, hkv, d)
+    key, value = _rows(g, t, hkv, d), _rows(g, t, hkv, d)
+    around = torch.full((t + 2,), 16, dtype=torch.int64)
+    around[1:-1] = 23 + torch.arange(t)
+    if t > 2:
+        around[3], around[4], around[5] = -(2**63), 2**63 - 1, 16 * nb
+    slots = around[1:-1]
+    want, table = oracle.append_reference(cache, scales, key, value, slots)
+    dc, ds = cache.clone().to(gpu), scales.clone().to(gpu)
+    view = around.to(gpu)[1:-1]
+    assert view.data_ptr() % 16 == 8
+    append_kv(key.to(gpu), value.to(gpu), dc, view, block_scales=ds)
+    torch.cuda.synchronize()
+    assert torch.equal(dc.cpu().view(torch.uint8), want.view(torch.uint8))
+    assert torch.equal(ds.cpu().nan_to_num(-1.0), table.nan_to_num(-1.0))
+
+
+@pytest.mark.gpu
 def test_append_nothing(gpu):
     from arctic_platform_amd import append_kv
 
