@@ -33,7 +33,9 @@ namespace fca {
 // Direct-to-LDS loads: a wave copies `PIECES` KB of a block to LDS as they lie.  An instruction moves 16
 // bytes per lane to M0 + 16 * lane, and its immediate offset counts on both sides.  Written as assembly so
 // that the compiler's wait insertion does not know of the loads (it would drain them before every LDS
-// read); loads it does not know of only make its own waits more conservative.
+// read); loads it does not know of only make its own waits more conservative.  Nor does its hazard
+// check look inside: a load to LDS follows a write of M0, and of a scalar register by a vector
+// instruction, by at least one and five wait states, which the s_nop provides.
 __device__ inline unsigned lds_address(const void* p) {
   return __builtin_amdgcn_readfirstlane((unsigned)(size_t)((__attribute__((address_space(3))) void*)(p)));
 }
@@ -41,7 +43,7 @@ template <int PIECES, bool STREAM>
 __device__ inline void block_to_lds(const char* block, int lane_off, unsigned lds) {
   static_assert(PIECES == 1 || PIECES == 2 || PIECES == 4, "");
 #define FCA_TO_LDS(MORE, NT) \
-  asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" NT MORE : : "v"(lane_off), "s"(block), "s"(lds) : "memory", "m0")
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %0, %1" NT MORE : : "v"(lane_off), "s"(block), "s"(lds) : "memory", "m0")
 #define FCA_PIECE(OFF, NT) "\n\tglobal_load_lds_dwordx4 %0, %1 offset:" OFF NT
   if constexpr (STREAM) {
     if constexpr (PIECES == 1) FCA_TO_LDS("", " nt");
