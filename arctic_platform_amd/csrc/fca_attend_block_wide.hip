@@ -47,12 +47,12 @@ __device__ inline void block_to_lds(const char* block, int lane_off, unsigned ld
 #define FCA_PIECE(OFF, NT) "\n\tglobal_load_lds_dwordx4 %0, %1 offset:" OFF NT
   if constexpr (STREAM) {
     if constexpr (PIECES == 1) FCA_TO_LDS("", " nt");
-    if constexpr (PIECES == 2) FCA_TO_LDS(FCA_PIECE("1024", " nt"), " nt");
-    if constexpr (PIECES == 4) FCA_TO_LDS(FCA_PIECE("1024", " nt") FCA_PIECE("2048", " nt") FCA_PIECE("3072", " nt"), " nt");
+    if constexpr (PIECES == 2) FCA_TO_LDS(FCA_PIECE("1*1024", " nt"), " nt");
+    if constexpr (PIECES == 4) FCA_TO_LDS(FCA_PIECE("1*1024", " nt") FCA_PIECE("2*1024", " nt") FCA_PIECE("3*1024", " nt"), " nt");
   } else {
     if constexpr (PIECES == 1) FCA_TO_LDS("", "");
-    if constexpr (PIECES == 2) FCA_TO_LDS(FCA_PIECE("1024", ""), "");
-    if constexpr (PIECES == 4) FCA_TO_LDS(FCA_PIECE("1024", "") FCA_PIECE("2048", "") FCA_PIECE("3072", ""), "");
+    if constexpr (PIECES == 2) FCA_TO_LDS(FCA_PIECE("1*1024", ""), "");
+    if constexpr (PIECES == 4) FCA_TO_LDS(FCA_PIECE("1*1024", "") FCA_PIECE("2*1024", "") FCA_PIECE("3*1024", ""), "");
   }
 #undef FCA_PIECE
 #undef FCA_TO_LDS
