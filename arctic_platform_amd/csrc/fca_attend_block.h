@@ -14,6 +14,17 @@ constexpr int kNanTag = 1;
 // overflows, each alone is a bf16 number.
 constexpr float kHuge = 0x1p120f;
 
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+// 8 e4m3 codes -> 8 halves (every e4m3 value is one, so the conversion is exact).
+__device__ inline f16x8 fp8x8_to_f16(i32x2 w) {
+  const f16x2 a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w[0], 1.0f, false);
+  const f16x2 b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w[0], 1.0f, true);
+  const f16x2 c = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w[1], 1.0f, false);
+  const f16x2 d = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w[1], 1.0f, true);
+  return f16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+
 // 0xff in every byte of a dword of codes that holds a NaN (0x7f or 0xff).
 __device__ inline unsigned nan_bytes(unsigned w) {
   const unsigned x = (w & 0x7f7f7f7fu) + 0x01010101u;  // bit 7 of a byte: its magnitude was 0x7f
@@ -68,6 +79,74 @@ __device__ inline V without_nans(V raw, int& found) {
     found |= bad;
   }
   return raw;
+}
+
+// ---- softmax of one query row (a lane and the one 32 away hold one) ----------------------------
+// The value product takes the weights p * s_v as halves: 11 significant bits where bf16 has 8, at the
+// same rate of the matrix cores.  What is left of the error of a bf16 output is the rounding of the
+// output: 0.0015 to 0.0017 relative to the definition in 64 bits at five sizes, as with fp32 weights
+// (with bf16 weights 0.0021 to 0.0022).  A half spans 2^-24 to 2^15, so the weights have a reference
+// of their own next to that of the exponentials: the largest log2(p) + log2(s_v) the row has met.
+// The largest weight is then about 2^kWeightBits; one 2^-21 of it still has 11 bits, and what is lost
+// of a smaller one is below 2^-32 of the largest, whatever the scales of the blocks are.  Measured
+// against bf16 weights with one reference: 0 to 3 % of a call (verify steps 52.5 -> 53.9 us the most).
+constexpr float kWeightBits = 7.f;  // + kRescaleSlack = 15: a half ends at 65504
+struct RowState {
+  float m, w;  // references (log2 domain): of the scaled scores, of those plus log2 of the V scale
+  float g;     // weight = exp2(score - m) * V scale * g
+  float l;     // running sum of exp2(score - m)
+};
+__device__ inline RowState empty_row() { return RowState{-INFINITY, -INFINITY, 1.f, 0.f}; }
+// log2 of a V scale, kept where the writer's scales are: the factor g stays a normal number.
+__device__ inline float scale_log2(float vs) { return fminf(fmaxf(fast_log2(vs), (float)(kScaleExpMin - 127)), (float)(kScaleExpMax - 127)); }
+
+// Scores of a tile -> weights, register r holding token 16 * (r / 8) + 8 * h + r % 8 of the tile; ks, vs, lv:
+// K scale (log2 domain), V scale and its log2 of the tile's two blocks.  RAGGED: registers of tokens from
+// `lim` on (counted from 8 * h) are masked.
+template <bool RAGGED, int NDB>
+__device__ inline void weigh_tile(RowState& row, bool first, f32x16 sr, const float (&ks)[2], const float (&vs)[2], const float (&lv)[2], int lim,
+                                  f32x16 (&acc)[NDB], f16x8 (&weights)[2]) {
+  if constexpr (RAGGED) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r)
+      if (16 * (r >> 3) + (r & 7) >= lim) sr[r] = -INFINITY;
+  }
+  float mx[2];
+#pragma unroll
+  for (int blk = 0; blk < 2; ++blk) {
+    mx[blk] = sr[8 * blk];
+#pragma unroll
+    for (int r = 1; r < 8; ++r) mx[blk] = fmaxf(mx[blk], sr[8 * blk + r]);
+    mx[blk] *= ks[blk];  // (the scales are positive, so the maximum of the scaled scores is a scaled maximum)
+  }
+  float mtile = fmaxf(mx[0], mx[1]), wtile = fmaxf(mx[0] + lv[0], mx[1] + lv[1]);
+  mtile = fmaxf(mtile, other_half(mtile));
+  wtile = fmaxf(wtile, other_half(wtile));
+  // The references move (and sum and accumulators are rescaled) only when a maximum rises more than
+  // kRescaleSlack above its own.
+  if (first) row.m = mtile, row.w = wtile, row.g = fast_exp2(mtile - wtile + kWeightBits);
+  if (__ballot(mtile > row.m + kRescaleSlack || wtile > row.w + kRescaleSlack) != 0) {
+    const float m_new = fmaxf(row.m, mtile), w_new = fmaxf(row.w, wtile);
+    const float alpha = fast_exp2(row.w - w_new);
+    row.l *= fast_exp2(row.m - m_new);
+    row.m = m_new, row.w = w_new;
+    row.g = fast_exp2(m_new - w_new + kWeightBits);
+#pragma unroll
+    for (int db = 0; db < NDB; ++db)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[db][r] *= alpha;
+  }
+  const float factor[2] = {vs[0] * row.g, vs[1] * row.g};
+  float sum = 0.f;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) {
+    float e = fast_exp2(__builtin_fmaf(sr[r], ks[r >> 3], -row.m));
+    // (a masked score times a scale of zero is no number)
+    if (RAGGED && sr[r] == -INFINITY) e = 0.f;
+    sum += e;
+    weights[r >> 3][r & 7] = (_Float16)(e * factor[r >> 3]);
+  }
+  row.l += sum;
 }
 
 // 64-row items (head sizes 64 and 128) and head size 256: fca_attend_block_wide.hip

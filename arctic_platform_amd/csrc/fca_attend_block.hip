@@ -7,9 +7,9 @@
 //
 // A 32-token tile covers two blocks, and the accumulator registers 0-7 and 8-15 of a lane hold the
 // tokens of the first and the second: the K scale is one of two wave-uniform factors of the
-// exponent's fused multiply-add, the V scale one multiplication of a probability before it is
-// rounded to bf16 for the value product (that rounding is relative, so the scale costs no
-// precision).  The codes go through the matrix cores as bf16, which holds every e4m3 value exactly.
+// exponent's fused multiply-add, the V scale one factor of a probability before it is rounded to a
+// half for the value product (see RowState).  The codes go through the matrix cores as bf16 (K, next to
+// bf16 query rows) and as halves (V), both of which hold every e4m3 value exactly.
 // (As codes, with the query row split into two rows of codes, a product is no faster, and the 8-bit
 // matrix instructions drop products below 2^-13 of the largest one they add.)
 //
@@ -185,15 +185,17 @@ __global__ __launch_bounds__(kThreads, block_workgroups<D>()) void fca_attend_bl
     // (its own token and what is before it); all members end inside the last tile.
     int sees;
     f32x16 acc[NDB];
-    float mrow, lrow;  // reference maximum (scaled, log2 domain) and running sum
-    float ks;          // K scale of the lane's block, times softmax scale and log2(e)
+    RowState row;
+    float ks;  // K scale of the lane's block, times softmax scale and log2(e)
+    float lv;  // log2 of its V scale
   };
   auto begin_item = [&](Item& it) {
     it.tok_len = __builtin_amdgcn_readfirstlane(r0.z);
     it.nblk = (it.tok_len + kBlock - 1) / kBlock;
     it.sees = __builtin_amdgcn_readfirstlane(r1.w);
     it.ks = my_scale.x * (p.scale * kLog2e);
-    it.mrow = -INFINITY, it.lrow = 0.f;
+    it.lv = scale_log2(my_scale.y);
+    it.row = empty_row();
 #pragma unroll
     for (int db = 0; db < NDB; ++db)
 #pragma unroll
@@ -204,12 +206,13 @@ __global__ __launch_bounds__(kThreads, block_workgroups<D>()) void fca_attend_bl
   auto compute_tile = [&](Item& it, const KT& kt, const VT& vt, int ti, auto ragged) {
     constexpr bool RAGGED = decltype(ragged)::value;
     const int tok0 = ti * kTile;
-    float ks[2], vs[2];
+    float ks[2], vs[2], lv[2];
 #pragma unroll
     for (int blk = 0; blk < 2; ++blk) {
       const int b = min(2 * ti + blk, it.nblk - 1);
       ks[blk] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(it.ks), b));
       vs[blk] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(my_scale.y), b));
+      lv[blk] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(it.lv), b));
     }
     f32x16 sr;
 #pragma unroll
@@ -220,47 +223,9 @@ __global__ __launch_bounds__(kThreads, block_workgroups<D>()) void fca_attend_bl
       const bf16x8 a = (i & 1) ? fp8x8_to_bf16(w[2], w[3]) : fp8x8_to_bf16(w[0], w[1]);
       sr = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, qreg[i], sr, 0, 0, 0);
     }
-    // register r holds token 16 * (r / 8) + 8 * h + r % 8 of the tile, for this lane's query row
-    if constexpr (RAGGED) {
-      const int lim = (it.sees > 0 ? min(it.tok_len, it.sees + row_member) : it.tok_len) - tok0 - 8 * h;
-#pragma unroll
-      for (int r = 0; r < 16; ++r)
-        if (16 * (r >> 3) + (r & 7) >= lim) sr[r] = -INFINITY;
-    }
-    float mx[2];
-#pragma unroll
-    for (int blk = 0; blk < 2; ++blk) {
-      mx[blk] = sr[8 * blk];
-#pragma unroll
-      for (int r = 1; r < 8; ++r) mx[blk] = fmaxf(mx[blk], sr[8 * blk + r]);
-    }
-    // the scales are positive, so the maximum of the scaled scores is a scaled maximum.  The
-    // reference of the exponentials moves (and the accumulators are rescaled) only when a row's
-    // maximum rises more than kRescaleSlack above it.
-    float mtile = fmaxf(mx[0] * ks[0], mx[1] * ks[1]);
-    mtile = fmaxf(mtile, other_half(mtile));
-    if (ti == 0) it.mrow = mtile;
-    if (__ballot(mtile > it.mrow + kRescaleSlack) != 0) {
-      const float mnew = fmaxf(it.mrow, mtile);
-      const float alpha = fast_exp2(it.mrow - mnew);
-      it.lrow *= alpha;
-      it.mrow = mnew;
-#pragma unroll
-      for (int db = 0; db < NDB; ++db)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) it.acc[db][r] *= alpha;
-    }
-    float sum = 0.f;
-    bf16x8 pb[2];  // probabilities of the tile, times their V scale, as B operands
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      float e = fast_exp2(__builtin_fmaf(sr[r], ks[r >> 3], -it.mrow));
-      // (a masked score times a scale of zero is no number)
-      if (RAGGED && sr[r] == -INFINITY) e = 0.f;
-      sum += e;
-      pb[r >> 3][r & 7] = (__bf16)(e * vs[r >> 3]);
-    }
-    it.lrow += sum;
+    const int lim = (it.sees > 0 ? min(it.tok_len, it.sees + row_member) : it.tok_len) - tok0 - 8 * h;
+    f16x8 pb[2];  // weights of the tile as B operands
+    weigh_tile<RAGGED>(it.row, ti == 0, sr, ks, vs, lv, lim, it.acc, pb);
     // (`run`: the last tile of a query run, whose rows see different numbers of its tokens)
     const bool run = RAGGED && it.sees > 0;
     int nans = 0;
@@ -276,7 +241,7 @@ __global__ __launch_bounds__(kThreads, block_workgroups<D>()) void fca_attend_bl
 #pragma unroll
         for (int db = 2 * pair; db < 2 * pair + 2; ++db) {
           const i32x2 w = value_codes(raw, db);
-          it.acc[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fp8x8_to_bf16(w[0], w[1]), pb[blk], it.acc[db], 0, 0, 0);
+          it.acc[db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fp8x8_to_f16(w), pb[blk], it.acc[db], 0, 0, 0);
         }
       }
     // A NaN among the values of such a tile must not reach the rows that do not see its token (0 * NaN),
@@ -311,11 +276,11 @@ __global__ __launch_bounds__(kThreads, block_workgroups<D>()) void fca_attend_bl
   // Write the partial of the item just attended: live rows go to `prow` (-1: a dead row), through a
   // wave-private strip of LDS so that they leave as whole rows; `tag` rides in the row's scale.
   auto write_partial = [&](Item& it, int64_t prow, int live_rows, int tag) {
-    const float l = it.lrow + other_half(it.lrow);
+    const float l = it.row.l + other_half(it.row.l);
     // an item half of which nobody attended here (the other wave of the pair took all of it)
     // leaves an empty partial: log-sum-exp -inf, weight 0 in the merge
     const float inv = l == 0.f ? 0.f : 1.f / l;
-    stage_partial_row<D, STREAM>(strip, m, h, it.acc, inv, prow, (it.mrow + fast_log2(l)) * kLn2, p.partial_lse, l != l ? kNanTag : tag);
+    stage_partial_row<D, STREAM>(strip, m, h, it.acc, inv / it.row.g, prow, (it.row.m + fast_log2(l)) * kLn2, p.partial_lse, l != l ? kNanTag : tag);
     __builtin_amdgcn_wave_barrier();
     store_partial_rows<D, STREAM>(strip, live_rows, lane, p.partial_out);
     __builtin_amdgcn_wave_barrier();

@@ -204,9 +204,10 @@ __global__ __launch_bounds__(128, 2) void fca_attend_block_wide_kernel(AttendPar
     const int row_member = row_tile ? member_of[1] : member_of[0], row_head = row_tile ? head_of[1] : head_of[0];
     const bool has_rows = row_tile == 0 || mcnt * G > 32;
     const float ks_lane = my_scale.x * (p.scale * kLog2e);  // K scale of the lane's block, log2 domain
+    const float lv_lane = scale_log2(my_scale.y);
 
     f32x16 acc[NDB];
-    float mrow = -INFINITY, lrow = 0.f;  // reference maximum (scaled, log2 domain) and running sum
+    RowState state = empty_row();
 #pragma unroll
     for (int db = 0; db < NDB; ++db)
 #pragma unroll
@@ -215,12 +216,13 @@ __global__ __launch_bounds__(128, 2) void fca_attend_block_wide_kernel(AttendPar
     auto compute_tile = [&](int ti, auto ragged) {
       constexpr bool RAGGED = decltype(ragged)::value;
       const int tok0 = ti * kTile;
-      float ks[2], vs[2];
+      float ks[2], vs[2], lv[2];
 #pragma unroll
       for (int blk = 0; blk < 2; ++blk) {
         const int b = min(2 * ti + blk, nblk - 1);
         ks[blk] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(ks_lane), b));
         vs[blk] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(my_scale.y), b));
+        lv[blk] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(lv_lane), b));
       }
       // (the fences keep reads of LDS together in front of the arithmetic they feed, V's in front of the
       // softmax: left alone the compiler reads one piece, waits for it, and reads the next)
@@ -244,46 +246,9 @@ __global__ __launch_bounds__(128, 2) void fca_attend_block_wide_kernel(AttendPar
         for (int blk = 0; blk < 2; ++blk)
           vw[blk][db] = *reinterpret_cast<const i32x2*>(&ring[slot][0] + v_off + (blk * D + 32 * db) * kBlock);
       __builtin_amdgcn_sched_barrier(0);
-      // register r holds token 16 * (r / 8) + 8 * h + r % 8 of the tile, for this lane's query row
-      if constexpr (RAGGED) {
-        const int lim = (sees > 0 ? min(tok_len, sees + row_member) : tok_len) - tok0 - 8 * h;
-#pragma unroll
-        for (int r = 0; r < 16; ++r)
-          if (16 * (r >> 3) + (r & 7) >= lim) sr[r] = -INFINITY;
-      }
-      float mx[2];
-#pragma unroll
-      for (int blk = 0; blk < 2; ++blk) {
-        mx[blk] = sr[8 * blk];
-#pragma unroll
-        for (int r = 1; r < 8; ++r) mx[blk] = fmaxf(mx[blk], sr[8 * blk + r]);
-      }
-      // the scales are positive, so the maximum of the scaled scores is a scaled maximum; the reference
-      // of the exponentials moves only when a row's maximum rises more than kRescaleSlack above it
-      float mtile = fmaxf(mx[0] * ks[0], mx[1] * ks[1]);
-      mtile = fmaxf(mtile, other_half(mtile));
-      if (ti == 0) mrow = mtile;
-      if (__ballot(mtile > mrow + kRescaleSlack) != 0) {
-        const float mnew = fmaxf(mrow, mtile);
-        const float alpha = fast_exp2(mrow - mnew);
-        lrow *= alpha;
-        mrow = mnew;
-#pragma unroll
-        for (int db = 0; db < NDB; ++db)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) acc[db][r] *= alpha;
-      }
-      float sum = 0.f;
-      bf16x8 pb[2];  // probabilities of the tile, times their V scale, as B operands
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        float e = fast_exp2(__builtin_fmaf(sr[r], ks[r >> 3], -mrow));
-        // (a masked score times a scale of zero is no number)
-        if (RAGGED && sr[r] == -INFINITY) e = 0.f;
-        sum += e;
-        pb[r >> 3][r & 7] = (__bf16)(e * vs[r >> 3]);
-      }
-      lrow += sum;
+      const int lim = (sees > 0 ? min(tok_len, sees + row_member) : tok_len) - tok0 - 8 * h;
+      f16x8 pb[2];  // weights of the tile as B operands
+      weigh_tile<RAGGED>(state, ti == 0, sr, ks, vs, lv, lim, acc, pb);
       // (`run`: the last tile of a query run, whose rows see different numbers of its tokens)
       const bool run = RAGGED && sees > 0;
       int nans = 0;
@@ -296,7 +261,7 @@ __global__ __launch_bounds__(128, 2) void fca_attend_block_wide_kernel(AttendPar
             w = first_codes(w, tok_len - (tok0 + 16 * blk + 8 * h));
             if (run) w = without_nans(w, nans);
           }
-          acc[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fp8x8_to_bf16(w[0], w[1]), pb[blk], acc[db], 0, 0, 0);
+          acc[db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fp8x8_to_f16(w), pb[blk], acc[db], 0, 0, 0);
         }
       // A NaN among the values of such a tile must not reach the rows that do not see its token (0 * NaN),
       // so it was left out of the product.  Where a row does see one, the product of (huge where the
@@ -351,8 +316,8 @@ __global__ __launch_bounds__(128, 2) void fca_attend_block_wide_kernel(AttendPar
     // every other four channels of its row; after a swap with the lane 32 away it has eight adjacent
     // ones.  (Through a strip of LDS, so that rows leave whole, it took 3 us an item.)
     {
-      const float l = lrow + other_half(lrow);
-      const float inv = 1.f / l;
+      const float l = state.l + other_half(state.l);
+      const float inv = 1.f / l / state.g;  // (l * g could overflow where all V scales are small)
       float amax = 0.f;
 #pragma unroll
       for (int db = 0; db < NDB; ++db)
@@ -368,7 +333,7 @@ __global__ __launch_bounds__(128, 2) void fca_attend_block_wide_kernel(AttendPar
       const float k = inv / scale;  // exact: the scale is a power of two
       const int64_t prow = has_rows && row_member < mcnt ? ((int64_t)seq * p.max_partials + cur.ord) * p.num_q_heads + cur.kvh * G + row_head : -1;
       if (h == 0 && prow >= 0 && (!Tune::kChannels || wave == 0)) {
-        const f32x2 ls = {(mrow + fast_log2(l)) * kLn2, __uint_as_float(__float_as_uint(scale) | (l != l ? (unsigned)kNanTag : 0u))};
+        const f32x2 ls = {(state.m + fast_log2(l)) * kLn2, __uint_as_float(__float_as_uint(scale) | (l != l ? (unsigned)kNanTag : 0u))};
         if constexpr (STREAM) store8_coherent(p.partial_lse + 2 * prow, __builtin_bit_cast(uint64_t, ls));
         else *reinterpret_cast<f32x2*>(p.partial_lse + 2 * prow) = ls;
       }

@@ -5,7 +5,7 @@
 // emu::host_threads above 1, several at a time on host threads of their own (LDS is per host thread,
 // atomics are the host's), which is how the workgroups of a persistent grid meet on a GPU.  What the
 // kernels see of the GPU's data layouts (the operand and result registers of
-// mfma_f32_32x32x16_bf16, v_permlane32_swap, the fp8 conversions, direct-to-LDS loads) follows
+// mfma_f32_32x32x16_bf16 and _f16, v_permlane32_swap, the fp8 conversions, direct-to-LDS loads) follows
 // the instruction set.  It checks kernel logic: indices, rings, masks, the dealing of work, and,
 // with buffers placed against inaccessible pages by the caller, addresses.  It says nothing about
 // speed, about the memory model between workgroups, or about what the compiler makes of the code.
@@ -229,12 +229,14 @@ inline T readlane(T v, int l) {
 }
 
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
 typedef float f32x16_t __attribute__((ext_vector_type(16)));
 // D[i][j] += sum_k A[i][k] B[k][j], 32 x 32 x 16.  Lane (m, h): A row m, B column m, k = 8 h .. 8 h + 7;
 // D register r of lane (j, h): row 8 (r / 4) + 4 h + r % 4, column j.
-inline f32x16_t mfma_32x32x16_bf16(bf16x8_t a, bf16x8_t b, f32x16_t c, int, int, int) {
+template <class E, class V>
+inline f32x16_t mfma_32x32x16(V a, V b, f32x16_t c) {
   struct {
-    bf16x8_t a, b;
+    V a, b;
   } mine{a, b};
   auto st = wave_exchange(&mine, sizeof(mine));
   const int j = F->lane & 31, h = F->lane >> 5;
@@ -242,14 +244,17 @@ inline f32x16_t mfma_32x32x16_bf16(bf16x8_t a, bf16x8_t b, f32x16_t c, int, int,
     const int i = 8 * (r / 4) + 4 * h + (r % 4);
     double s = 0;
     for (int k = 0; k < 16; ++k) {
-      const __bf16* pa = reinterpret_cast<const __bf16*>(st[i + 32 * (k / 8)]);
-      const __bf16* pb = reinterpret_cast<const __bf16*>(st[j + 32 * (k / 8)] + 16);
-      s += (double)(float)pa[k % 8] * (double)(float)pb[k % 8];
+      E x, y;
+      memcpy(&x, st[i + 32 * (k / 8)] + 2 * (k % 8), 2);
+      memcpy(&y, st[j + 32 * (k / 8)] + 16 + 2 * (k % 8), 2);
+      s += (double)(float)x * (double)(float)y;
     }
     c[r] += (float)s;
   }
   return c;
 }
+inline f32x16_t mfma_32x32x16_bf16(bf16x8_t a, bf16x8_t b, f32x16_t c, int, int, int) { return mfma_32x32x16<__bf16>(a, b, c); }
+inline f32x16_t mfma_32x32x16_f16(f16x8_t a, f16x8_t b, f32x16_t c, int, int, int) { return mfma_32x32x16<_Float16>(a, b, c); }
 
 // ---- direct-to-LDS loads -------------------------------------------------------------------
 inline thread_local char lds_anchor;  // LDS "addresses" are offsets from here (static storage lies within 2 GiB of it)
@@ -372,9 +377,11 @@ inline int64_t min(int a, int64_t b) { return a < b ? a : b; }
 inline int64_t max(int a, int64_t b) { return a < b ? b : a; }
 namespace emu {
 typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
 [[noreturn]] inline void unsupported(const char* what) { fprintf(stderr, "emu: %s is not emulated\n", what); abort(); }
 }  // namespace emu
 #define __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8 emu::cvt_scalef32_pk_bf16_fp8_impl
+#define __builtin_amdgcn_cvt_scalef32_pk_f16_fp8 emu::cvt_scalef32_pk_f16_fp8_impl
 
 struct alignas(16) int4 { int x, y, z, w; };
 struct alignas(8) int2 { int x, y; };
@@ -471,6 +478,13 @@ inline bf16x2_t cvt_scalef32_pk_bf16_fp8_impl(int src, float scale, bool hi) {
   r[1] = (__bf16)(fp8_e4m3_to_float((w >> 8) & 255) * scale);
   return r;
 }
+inline f16x2_t cvt_scalef32_pk_f16_fp8_impl(int src, float scale, bool hi) {
+  const unsigned w = (unsigned)src >> (hi ? 16 : 0);
+  f16x2_t r;
+  r[0] = (_Float16)(fp8_e4m3_to_float(w & 255) * scale);
+  r[1] = (_Float16)(fp8_e4m3_to_float((w >> 8) & 255) * scale);
+  return r;
+}
 inline float cvt_f32_fp8(int src, int sel) { return fp8_e4m3_to_float(((unsigned)src >> (8 * sel)) & 255); }
 inline f32x2_t cvt_pk_f32_fp8(int src, bool hi) {
   const unsigned w = (unsigned)src >> (hi ? 16 : 0);
@@ -502,6 +516,7 @@ inline int cvt_pk_fp8_f32(float a, float b, int old, bool hi) {
 #define __builtin_amdgcn_readfirstlane(v) emu::readfirstlane(v)
 #define __builtin_amdgcn_readlane(v, l) emu::readlane(v, l)
 #define __builtin_amdgcn_mfma_f32_32x32x16_bf16 emu::mfma_32x32x16_bf16
+#define __builtin_amdgcn_mfma_f32_32x32x16_f16 emu::mfma_32x32x16_f16
 #define __builtin_amdgcn_exp2f(x) exp2f(x)
 #define __builtin_amdgcn_logf(x) log2f(x)
 #define __builtin_amdgcn_s_waitcnt(x) ((void)0)
