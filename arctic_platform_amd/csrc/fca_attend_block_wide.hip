@@ -378,8 +378,10 @@ hipError_t launch_attend_block_wide(const AttendParams& p, const fca_plan& plan,
   const int64_t max_tickets = L.max_items * plan.num_kv_heads;
   int per_cu = WideTuning<64>::kWorkgroups;
   if (plan.head_dim == 256) per_cu = WideTuning<256>::kWorkgroups;
-  // (the caller's cap counts workgroups of four waves)
-  int64_t grid = (int64_t)(max_workgroups > 0 && max_workgroups < cus ? max_workgroups : cus) * per_cu;
+  int64_t grid = (int64_t)cus * per_cu;
+  // The caller's cap leaves CUs to other streams, and a launch spreads over as many CUs as it has
+  // workgroups: it counts them as they are, of two waves here.
+  if (max_workgroups > 0 && max_workgroups < grid) grid = max_workgroups;
   if (grid > max_tickets) grid = max_tickets;
   if (grid < 1) grid = 1;
   // with sharing on, and but for query runs, a launch reads every KV block about once: past the caches

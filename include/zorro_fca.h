@@ -105,8 +105,9 @@ typedef struct fca_tensors {
                                   item is cut, and with it the last bit of a few outputs, never depends
                                   on timing: two launches on the same inputs give the same bits */
   int32_t max_workgroups;      /* > 0: the attention launch uses at most this many workgroups (four waves
-                                  each; two in the fp32 path), leaving the rest of the GPU to work on
-                                  other streams; 0: all */
+                                  each; two in the fp32 path and, over a block-scaled cache, with
+                                  64-row items or head_dim 256), leaving the rest of the GPU to work
+                                  on other streams; 0: all */
   int32_t tile_buffers;        /* 0: the kernel's own choice (two register tile buffers per wave in the
                                   32-row kernel).  3: three, for fp8 caches at head_dim 128 with
                                   rows_per_item 32 only (an fp8 tile is half the bytes of a bf16 one, so

@@ -349,8 +349,11 @@ inline void run_blocks(dim3 grid, dim3 block, const std::function<void()>& kerne
   F = nullptr;
 }
 
+inline std::atomic<unsigned> launched_blocks{0}, launched_threads{0};  // of the last launch
+
 template <class K>
 inline void launch(dim3 grid, dim3 block, K&& kernel) {
+  launched_blocks = grid.x * grid.y * grid.z, launched_threads = block.x * block.y * block.z;
   const std::function<void()> body = kernel;
   const unsigned nblocks = grid.x * grid.y * grid.z;
   std::atomic<unsigned> next{0};

@@ -15,3 +15,7 @@ extern "C" void emu_set_run_order(int order) { emu::run_order = order; }
 
 // Workgroups of a launch that run at the same time, each on a host thread of its own (1: one after the other).
 extern "C" void emu_set_host_threads(int n) { emu::host_threads = n < 1 ? 1 : n; }
+
+// Workgroups of the last launch, and threads of each.
+extern "C" unsigned emu_last_workgroups() { return emu::launched_blocks; }
+extern "C" unsigned emu_last_threads() { return emu::launched_threads; }
