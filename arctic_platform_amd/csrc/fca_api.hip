@@ -474,8 +474,11 @@ static int cache_rows_block(bool gather, const void* key_dev, const void* value_
   a.num_blocks = num_blocks;
   a.num_kv_heads = num_kv_heads;
   a.head_dim = head_dim;
-  // (the writer's workgroups look at every slot of a launch; the reader's grid stays within 31 bits)
-  const int32_t most = gather ? 1 << 24 : fca::kAppendTokens;
+  // The reader's grid stays within 31 bits.  The writer's call is one launch: which tokens begin a block,
+  // and which share one, is a matter of the whole call.
+  if (!gather && num_tokens > fca::kAppendMostTokens)
+    return fail(FCA_ERR_UNSUPPORTED, "num_tokens %d is more than one call takes (%d)", num_tokens, fca::kAppendMostTokens);
+  const int32_t most = gather ? 1 << 24 : fca::kAppendMostTokens;
   for (int32_t t0 = 0; t0 < num_tokens; t0 += most) {
     a.num_tokens = num_tokens - t0 < most ? num_tokens - t0 : most;
     a.key = static_cast<const char*>(key_dev) + 2 * (int64_t)t0 * token_stride;

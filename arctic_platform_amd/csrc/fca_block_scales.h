@@ -33,8 +33,8 @@ __host__ __device__ inline int scale_exp_for(float amax) {
   return e < kScaleExpMin ? kScaleExpMin : e > kScaleExpMax ? kScaleExpMax : e;
 }
 
-// tokens of one append launch (every workgroup looks at all their slots)
-constexpr int kAppendTokens = 32768;
+// tokens of one append call (every workgroup looks at all their slots, with 32-bit indices)
+constexpr int32_t kAppendMostTokens = 1 << 30;
 
 struct BlockCacheParams {
   const void* key;  // bf16 [T, Hkv, D]; written by the reader

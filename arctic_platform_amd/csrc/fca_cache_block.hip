@@ -255,14 +255,22 @@ __device__ inline void append_v_tile(const BlockCacheParams& p, const int* win, 
 // whose first token of the call is among them.  Which of its blocks that holds for, and which later
 // tokens belong to them, it finds by looking at all slots of the call: they are few next to the rows
 // (8 bytes a token against 4 D Hkv), come out of the L2, and nothing has to be known about their order.
+// Cutting a long call into launches that see their own slots only would make the rule for the scales
+// depend on where the cut falls.  A slot's block is looked up among the window's (at most 64) in a table
+// of kTable places: one read of LDS for almost every slot, where comparing with all of them grows with
+// their number (131072 tokens of 8 heads of 128: 263 us in order and 0.8 ms scattered; by comparing 332
+// and 2.5 ms, cut into launches of 32768 tokens 269 and 2.1 ms).
 constexpr int kMaxWindow = 64;
 constexpr int kAppendThreads = 512;  // at most
+constexpr int kTable = 256;          // (at most a quarter of it is taken, so every search ends)
+__device__ inline int place_of(int blk) { return (int)((unsigned)blk * 0x9E3779B1u >> 24); }
 template <int D>
 __global__ __launch_bounds__(kAppendThreads) void fca_append_block_kernel(BlockCacheParams p, int window, int heads, int head_groups) {
   __shared__ int cand[kMaxWindow];         // blocks of the window's tokens, each once
   __shared__ int win[kMaxWindow][kBlock];  // the call's last token at every offset of theirs, -1 = none
   __shared__ int foreign[kMaxWindow];      // the block has a token in front of the window
   __shared__ int num_cand;
+  __shared__ int table[kTable];            // a candidate's number + 1 at the first free place from its block's on, 0 = none
   const int tid = threadIdx.x, threads = blockDim.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int w = blockIdx.x / head_groups, h0 = (blockIdx.x - w * head_groups) * heads;
@@ -280,7 +288,14 @@ __global__ __launch_bounds__(kAppendThreads) void fca_append_block_kernel(BlockC
       if (j < lane && other == blk) leads = false;
     }
     const unsigned long long all = __ballot(leads);
-    if (leads) cand[__popcll(all & ((1ull << lane) - 1))] = blk;
+    for (int j = lane; j < kTable; j += 64) table[j] = 0;
+    __builtin_amdgcn_wave_barrier();
+    if (leads) {
+      const int c = __popcll(all & ((1ull << lane) - 1));
+      cand[c] = blk;
+      int at = place_of(blk);
+      while (atomicCAS(&table[at], 0, c + 1) != 0) at = (at + 1) % kTable;
+    }
     if (lane == 0) num_cand = __popcll(all);
   }
   for (int j = tid; j < window * kBlock; j += threads) (&win[0][0])[j] = -1;
@@ -305,20 +320,18 @@ __global__ __launch_bounds__(kAppendThreads) void fca_append_block_kernel(BlockC
       else if (t < p.num_tokens)
         slots[k][0] = p.slot_mapping[t];
     }
-    for (int c = 0; c < n; ++c) {
-      const uint64_t first = (uint64_t)cand[c] * kBlock;
 #pragma unroll
-      for (int k = 0; k < kScan; ++k) {
-        const int t = base + 2 * (k * threads + tid);
-        const uint64_t x = (uint64_t)slots[k][0] - first, y = (uint64_t)slots[k][1] - first;  // (a negative slot is far away)
-        if (x < kBlock) {
-          if (t < t0) foreign[c] = 1;
-          else atomicMax(&win[c][x], t);
-        }
-        if (y < kBlock) {
-          if (t + 1 < t0) foreign[c] = 1;
-          else atomicMax(&win[c][y], t + 1);
-        }
+    for (int k = 0; k < 2 * kScan; ++k) {
+      const int t = base + 2 * ((k >> 1) * threads + tid) + (k & 1);
+      const int64_t slot = slots[k >> 1][k & 1];
+      const uint64_t blk = (uint64_t)slot / kBlock;  // (a negative slot is far away)
+      for (int at = place_of((int)blk);; at = (at + 1) % kTable) {
+        const int c = table[at] - 1;
+        if (c < 0) break;
+        if ((uint64_t)cand[c] != blk) continue;
+        if (t < t0) foreign[c] = 1;
+        else atomicMax(&win[c][slot & (kBlock - 1)], t);
+        break;
       }
     }
   }

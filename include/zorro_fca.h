@@ -317,11 +317,11 @@ int fca_gather_kv(void* key_dev, void* value_dev, int64_t token_stride, int64_t 
  * (blocks are used again without being cleared); the tokens behind it have to be written in that
  * call or after it.  Writing a token again is allowed; the scale of a begun block never falls.
  * Tokens of one call may come in any order; of two with the same slot the later one is stored.
- * A negative slot is padding; a slot of a block beyond num_blocks is skipped like padding.  Calls
- * of more than 32768 tokens have the effect of successive calls of 32768.
+ * A negative slot is padding; a slot of a block beyond num_blocks is skipped like padding.  At most
+ * 2^30 tokens (FCA_ERR_UNSUPPORTED beyond).
  * slot_mapping, key, value, strides: as for fca_append_kv (bf16 rows).  block_scales:
  * [num_blocks, Hkv, 2] fp32, contiguous, 8-byte aligned.  Calls that touch one block must be in
- * stream order, and so must reads of it.  One launch per 32768 tokens, no workspace. */
+ * stream order, and so must reads of it.  One launch, no workspace. */
 int fca_append_kv_block_scaled(const void* key_dev, const void* value_dev, int64_t token_stride, int64_t head_stride,
                                int32_t num_tokens, int32_t num_kv_heads, int32_t head_dim, const int64_t* slot_mapping_dev,
                                void* k_cache_dev, void* v_cache_dev, int64_t kv_block_stride, int64_t kv_head_stride,
