@@ -32,6 +32,7 @@ EXPORTS = (
     "fca_suffix_pass",
     "fca_forest_pass",
     "fca_merge",
+    "fca_merge_dtype",
     "fca_decode_step",
     "fca_decode_step_static",
     "fca_append_kv",
@@ -177,6 +178,7 @@ def declare_signatures(lib: ctypes.CDLL) -> ctypes.CDLL:
     lib.fca_suffix_pass.argtypes = attend
     lib.fca_forest_pass.argtypes = attend
     lib.fca_merge.argtypes = [P(FcaPlan), VP, VP, VP, VP, I64, I64, I32, VP, VP]
+    lib.fca_merge_dtype.argtypes = [P(FcaPlan), I32, VP, VP, VP, VP, I64, I64, I32, VP, VP]
     lib.fca_decode_step.argtypes = [P(FcaPlan), P(FcaTensors), VP, VP, VP, VP, I64, I64, I32, VP, VP]
     lib.fca_decode_step_static.argtypes = [P(FcaPlan), P(FcaTensors), VP, VP, I64, I64, I32, VP, VP]
     lib.fca_append_kv.argtypes = [VP, VP, I64, I64, I32, I32, I32, VP, VP, VP, I64, I64, I32, VP, VP, VP]

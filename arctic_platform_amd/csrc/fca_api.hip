@@ -180,10 +180,13 @@ int run_merge(const fca_plan* p, const void* meta, const void* po, const float* 
   // whole 16-byte stores when every 8-channel group of out is 16-byte aligned
   const int64_t esz = out_dtype == FCA_F32 ? 4 : 2;
   m.vector_out = !(reinterpret_cast<uintptr_t>(out) & 15) && (oss * esz) % 16 == 0 && (ohs * esz) % 16 == 0;
-  // Few rows that can have many partials, after attention over a block-scaled cache: a workgroup each
-  // (32 rows of 128 partials 12 -> 6 us; 4096 rows of 36 would take 16.6 us against 14.1, so from
-  // four rows per CU on a wave or less each; the other caches keep their order of summation).
-  const bool few_long = block_scaled && m.max_partials >= 16 && (int64_t)m.num_seqs * m.num_q_heads <= 1024;
+  // Few rows that can have many partials, after attention over a block-scaled cache: a workgroup each, of
+  // which all but one wave leave where a row has few (fca_merge_long.hip; the other caches keep their
+  // order of summation).  Up to one row per CU that loses nowhere, whatever the rows have of the partials
+  // they could have: 32 rows, D 128: 1 partial 3.0 us against 3.3 with a wave or less per row,
+  // 16 2.8 against 3.1, 128 4.9 against 9.3; 256 rows: 3.0 / 3.2, 2.9 / 3.2, 6.3 / 11.9.  Beyond, rows of
+  // few partials pay for the waves that leave (1024 rows of D 64: 1 partial 3.8 against 3.2).
+  const bool few_long = block_scaled && m.max_partials >= 16 && (int64_t)m.num_seqs * m.num_q_heads <= 256;
   hipError_t e = few_long ? fca::launch_merge_long(m, static_cast<hipStream_t>(stream))
                           : fca::launch_merge(m, static_cast<hipStream_t>(stream));
   return e == hipSuccess ? FCA_OK : hip_fail(e, "merge launch");
@@ -321,6 +324,15 @@ int fca_merge(const fca_plan* plan, const void* meta_dev, const void* partial_ou
               void* stream) {
   return run_merge(plan, meta_dev, partial_out_dev, partial_lse_dev, out_dev, out_seq_stride, out_head_stride, out_dtype,
                    lse_dev, stream);
+}
+
+int fca_merge_dtype(const fca_plan* plan, int32_t kv_dtype, const void* meta_dev, const void* partial_out_dev,
+                    const float* partial_lse_dev, void* out_dev, int64_t out_seq_stride, int64_t out_head_stride,
+                    int32_t out_dtype, float* lse_dev, void* stream) {
+  if (kv_dtype != FCA_BF16 && kv_dtype != FCA_FP8_E4M3 && kv_dtype != FCA_FP8_E4M3_BLOCK)
+    return fail(FCA_ERR_UNSUPPORTED, "kv_dtype %d has no separate merge (bf16, fp8 e4m3 or block-scaled fp8 e4m3)", kv_dtype);
+  return run_merge(plan, meta_dev, partial_out_dev, partial_lse_dev, out_dev, out_seq_stride, out_head_stride, out_dtype,
+                   lse_dev, stream, false, kv_dtype == FCA_FP8_E4M3_BLOCK);
 }
 
 int fca_decode_step(const fca_plan* plan, const fca_tensors* t, void* meta_dev, void* partial_out_dev,

@@ -3,10 +3,12 @@
 //
 // The merge of fca_merge.hip gives a row at most one wave; with the 128 partials of a sequence of
 // 131072 tokens that is eight round trips to memory one after the other, and a single sequence of 32
-// query heads occupies 8 of 256 CUs (12 us measured, against 44 us of the attention in front of it).
+// query heads occupies 8 of 256 CUs (9.3 us, against 44 us of the attention in front of it).
 // Here 2048 / D groups of D / 8 lanes take every (2048 / D)-th partial of the row each, four at a
 // time, all loads of a batch in flight together, and combine in registers and LDS: one round trip for
-// up to 64 partials at D = 128.  Partial rows, tags and NaN rules are those of fca_merge.hip, to
+// up to 64 partials at D = 128 (4.9 us for those 128).  How many partials a row has is known here, not
+// where the kernel is chosen: a row that one wave covers in one batch is left to one wave (2.8 us at 16
+// partials).  Partial rows, tags and NaN rules are those of fca_merge.hip, to
 // which the block-scaled cache adds that a second partial carries a tag of its own where its row is
 // no number (fca_attend_block.h).
 #include <hip/hip_bf16.h>
@@ -45,12 +47,17 @@ __device__ inline void add_running(Running& r, const Running& o) {
 template <int D>
 __global__ __launch_bounds__(256) void fca_merge_long_kernel(MergeParams p) {
   constexpr int LPS = D / 8;          // lanes per share of a row
-  constexpr int SHARES = 256 / LPS, B = 4;
+  constexpr int B = 4;
+  constexpr int WAVE_SHARES = 64 / LPS;
   __shared__ Running part[4][LPS];
   __shared__ int part_stray[4];
   const int row = blockIdx.x, s = row / p.num_q_heads, hq = row - s * p.num_q_heads;
   const int tid = threadIdx.x, sub = tid % LPS, share = tid / LPS, wave = tid >> 6, lane = tid & 63;
   const int np = p.seq_npart[s];
+  // a row that one wave covers in one batch is that wave's alone
+  const bool one_wave = np <= B * WAVE_SHARES;
+  if (one_wave && wave != 0) return;
+  const int shares = one_wave ? WAVE_SHARES : 4 * WAVE_SHARES;
   const int64_t base = (int64_t)s * p.max_partials;
   const _Float16* rows = static_cast<const _Float16*>(p.partial_out);
   const float2v* lse_scale = reinterpret_cast<const float2v*>(p.partial_lse);
@@ -59,19 +66,19 @@ __global__ __launch_bounds__(256) void fca_merge_long_kernel(MergeParams p) {
 #pragma unroll
   for (int e = 0; e < 8; ++e) r.acc[e] = 0.f;
   int stray = 0;
-  for (int i0 = share; i0 < np; i0 += B * SHARES) {
+  for (int i0 = share; i0 < np; i0 += B * shares) {
     float2v ls[B];
     half8 o[B];
 #pragma unroll
     for (int j = 0; j < B; ++j) {  // (past the row's last partial: that one again, at weight 0)
-      const int64_t pr = (base + min(i0 + j * SHARES, np - 1)) * p.num_q_heads + hq;
+      const int64_t pr = (base + min(i0 + j * shares, np - 1)) * p.num_q_heads + hq;
       ls[j] = __builtin_nontemporal_load(lse_scale + pr);
       o[j] = __builtin_nontemporal_load(reinterpret_cast<const half8*>(rows + pr * D + sub * 8));
     }
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int j = 0; j < B; ++j) {
-      if (i0 + j * SHARES >= np) ls[j] = float2v{-INFINITY, 1.f};
+      if (i0 + j * shares >= np) ls[j] = float2v{-INFINITY, 1.f};
       const unsigned tag = __float_as_uint(ls[j][1]) & 0x007fffffu;
       add_partial(r, ls[j][0], __uint_as_float(__float_as_uint(ls[j][1]) & 0xff800000u), o[j]);
       if (tag == 0) continue;
@@ -96,14 +103,18 @@ __global__ __launch_bounds__(256) void fca_merge_long_kernel(MergeParams p) {
     stray |= __shfl_xor(stray, off);
     add_running(r, x);
   }
-  if (lane < LPS) part[wave][lane] = r;
-  if (lane == 0) part_stray[wave] = stray;
-  __syncthreads();
+  if (!one_wave) {
+    if (lane < LPS) part[wave][lane] = r;
+    if (lane == 0) part_stray[wave] = stray;
+    __syncthreads();
+  }
   if (tid >= LPS) return;
+  if (!one_wave) {
 #pragma unroll
-  for (int w = 1; w < 4; ++w) {
-    add_running(r, part[w][sub]);
-    stray |= part_stray[w];
+    for (int w = 1; w < 4; ++w) {
+      add_running(r, part[w][sub]);
+      stray |= part_stray[w];
+    }
   }
   // input the builder had to clamp makes every output NaN, as in fca_merge.hip
   const bool flagged = p.header[H_ERROR] != 0 || stray != 0;

@@ -167,6 +167,7 @@ def prefix_pass(q, kv_cache, meta: ForestMetadata, scale, k_scale=None, v_scale=
     """Shared-node work items only; fills their slots of the partial buffers."""
     lib = _lib.load_library()
     t = _tensors(q, kv_cache, meta, scale, k_scale, v_scale, block_scales=block_scales)
+    meta.block_scaled = block_scales is not None
     with on_device(q.device):
         _lib.check(
             lib.fca_prefix_pass(
@@ -180,6 +181,7 @@ def suffix_pass(q, kv_cache, meta: ForestMetadata, scale, k_scale=None, v_scale=
     """Private-leaf work items only; fills their slots of the partial buffers."""
     lib = _lib.load_library()
     t = _tensors(q, kv_cache, meta, scale, k_scale, v_scale, block_scales=block_scales)
+    meta.block_scaled = block_scales is not None
     with on_device(q.device):
         _lib.check(
             lib.fca_suffix_pass(
@@ -193,6 +195,7 @@ def forest_pass(q, kv_cache, meta: ForestMetadata, scale, k_scale=None, v_scale=
     """Shared and private work items in one launch; fills every live partial slot."""
     lib = _lib.load_library()
     t = _tensors(q, kv_cache, meta, scale, k_scale, v_scale, block_scales=block_scales)
+    meta.block_scaled = block_scales is not None
     with on_device(q.device):
         _lib.check(
             lib.fca_forest_pass(
@@ -203,15 +206,16 @@ def forest_pass(q, kv_cache, meta: ForestMetadata, scale, k_scale=None, v_scale=
 
 
 def merge_partials(meta: ForestMetadata, q_like, out=None, return_lse=True, out_dtype=None):
-    """Log-sum-exp merge of the partial buffers into ``out`` (and ``lse``)."""
+    """Log-sum-exp merge of the partial buffers into ``out`` (and ``lse``): what ``forest_cascade_decode``
+    gives for the cache that the passes before it attended over, bit for bit with ``meta.reproducible``."""
     if meta.partial_out.dtype != torch.float16:
         raise TypeError("merge_partials reads the half-precision partial rows of the bf16 / fp8 passes; fp32 rows are merged inside forest_cascade_decode")
     lib = _lib.load_library()
     out, code = _out_args(q_like, meta, out, out_dtype)
     lse = torch.empty(meta.plan.num_seqs, meta.plan.num_q_heads, dtype=torch.float32, device=out.device) if return_lse else None
     _lib.check(
-        lib.fca_merge(
-            ctypes.byref(meta.plan), meta.meta.data_ptr(), meta.partial_out.data_ptr(), meta.partial_lse.data_ptr(),
+        lib.fca_merge_dtype(
+            ctypes.byref(meta.plan), _lib.FCA_FP8_E4M3_BLOCK if meta.block_scaled else _lib.FCA_BF16, meta.meta.data_ptr(), meta.partial_out.data_ptr(), meta.partial_lse.data_ptr(),
             out.data_ptr(), out.stride(0), out.stride(1), code, lse.data_ptr() if lse is not None else None,
             _stream_ptr(out.device),
         )

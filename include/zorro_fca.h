@@ -260,6 +260,12 @@ int fca_forest_pass(const fca_plan* plan, const fca_tensors* t, void* meta_dev,
 int fca_merge(const fca_plan* plan, const void* meta_dev, const void* partial_out_dev,
               const float* partial_lse_dev, void* out_dev, int64_t out_seq_stride, int64_t out_head_stride,
               int32_t out_dtype, float* lse_dev, void* stream);
+/* The same after passes over a cache of the given kv_dtype (not FCA_F32): the merge that fca_decode_step
+ * runs there, bit for bit.  After FCA_FP8_E4M3_BLOCK few rows that can have many partials are added in
+ * another order than by fca_merge, which also merges them (the last bits may differ). */
+int fca_merge_dtype(const fca_plan* plan, int32_t kv_dtype, const void* meta_dev, const void* partial_out_dev,
+                    const float* partial_lse_dev, void* out_dev, int64_t out_seq_stride, int64_t out_head_stride,
+                    int32_t out_dtype, float* lse_dev, void* stream);
 /* One layer's decode attention: prefix and suffix items in one launch, then the merge. */
 int fca_decode_step(const fca_plan* plan, const fca_tensors* t, void* meta_dev,
                     void* partial_out_dev, float* partial_lse_dev, void* out_dev, int64_t out_seq_stride,
