@@ -141,8 +141,8 @@ __device__ inline void weigh_tile(RowState& row, bool first, f32x16 sr, const fl
 #pragma unroll
   for (int r = 0; r < 16; ++r) {
     float e = fast_exp2(__builtin_fmaf(sr[r], ks[r >> 3], -row.m));
-    // (a masked score times a scale of zero is no number)
-    if (RAGGED && sr[r] == -INFINITY) e = 0.f;
+    // (by its place: minus infinity may be a score too, and times a scale of zero it is no number)
+    if (RAGGED && 16 * (r >> 3) + (r & 7) >= lim) e = 0.f;
     sum += e;
     weights[r >> 3][r & 7] = (_Float16)(e * factor[r >> 3]);
   }
