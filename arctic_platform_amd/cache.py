@@ -11,23 +11,11 @@ engine's attention backend, which is what this call replaces.
 
 from __future__ import annotations
 
-import contextlib
-
 import torch
 
 from . import _lib
-from .forest import _stream_ptr
+from .forest import _stream_ptr, on_device
 from .kv_layout import BLOCK_SIZE, block_scales_shape
-
-
-def on_device(device):
-    """A launch goes to the current device: makes ``device`` that for a call on another one's tensors."""
-    if device.type != "cuda" or device.index == torch._C._cuda_getDevice():
-        return _CURRENT
-    return torch.cuda.device(device)
-
-
-_CURRENT = contextlib.nullcontext()
 
 
 def check_block_scales(block_scales, kv_cache, k_scale, v_scale) -> None:
@@ -105,14 +93,15 @@ def _cache_rows(gather, key, value, kv_cache, slot_mapping, k_scale, v_scale, bl
             raise ValueError(f"{name} must be a contiguous fp32 tensor of shape [{hkv}]")
     lib = _lib.load_library()
     esz = kv_cache.element_size()
-    _lib.check(
-        (lib.fca_gather_kv if gather else lib.fca_append_kv)(
-            key.data_ptr(), value.data_ptr(), key.stride(0), key.stride(1), t, hkv, d, slot_mapping.data_ptr(),
-            kv_cache.data_ptr(), kv_cache.data_ptr() + kv_cache.stride(0) * esz, kv_cache.stride(1), kv_cache.stride(2),
-            code, k_scale.data_ptr() if k_scale is not None else None, v_scale.data_ptr() if v_scale is not None else None,
-            _stream_ptr(key.device),
+    with on_device(key.device):
+        _lib.check(
+            (lib.fca_gather_kv if gather else lib.fca_append_kv)(
+                key.data_ptr(), value.data_ptr(), key.stride(0), key.stride(1), t, hkv, d, slot_mapping.data_ptr(),
+                kv_cache.data_ptr(), kv_cache.data_ptr() + kv_cache.stride(0) * esz, kv_cache.stride(1), kv_cache.stride(2),
+                code, k_scale.data_ptr() if k_scale is not None else None, v_scale.data_ptr() if v_scale is not None else None,
+                _stream_ptr(key.device),
+            )
         )
-    )
 
 
 def _block_scaled_rows(gather, key, value, kv_cache, slot_mapping, block_scales) -> None:

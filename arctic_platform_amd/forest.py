@@ -12,6 +12,7 @@ are leading runs of physical block ids and the rule is applied level by level.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import dataclasses
 
@@ -26,6 +27,16 @@ ITEM_INTS = 8
 def _stream_ptr(device) -> int:
     # (the handle itself; building a Stream object around it takes several microseconds a call)
     return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if device.index is None else device.index)
+
+
+def on_device(device):
+    """A launch goes to the current device: makes ``device`` that for a call on another one's tensors."""
+    if device.type != "cuda" or device.index == torch._C._cuda_getDevice():
+        return _CURRENT
+    return torch.cuda.device(device)
+
+
+_CURRENT = contextlib.nullcontext()
 
 
 @dataclasses.dataclass
@@ -148,12 +159,13 @@ def rows_from_query_runs(query_start_loc: torch.Tensor, seq_lens: torch.Tensor, 
     if out is None:
         out = tuple(torch.empty(num_rows, dtype=torch.int32, device=seq_lens.device) for _ in range(3))
     row_table, row_lens, row_group = (t[:num_rows] for t in out)
-    _lib.check(
-        _lib.load_library().fca_rows_from_query_runs(
-            query_start_loc.data_ptr(), seq_lens.data_ptr(), num_reqs, num_rows, max_blocks,
-            row_table.data_ptr(), row_lens.data_ptr(), row_group.data_ptr(), _stream_ptr(seq_lens.device),
+    with on_device(seq_lens.device):
+        _lib.check(
+            _lib.load_library().fca_rows_from_query_runs(
+                query_start_loc.data_ptr(), seq_lens.data_ptr(), num_reqs, num_rows, max_blocks,
+                row_table.data_ptr(), row_lens.data_ptr(), row_group.data_ptr(), _stream_ptr(seq_lens.device),
+            )
         )
-    )
     return row_table, row_lens, row_group
 
 
@@ -259,30 +271,32 @@ def build_forest_metadata(
             kv_reread=row_group is not None if kv_reread is None else bool(kv_reread),
         )
     if row_table is not None:
+        with on_device(block_table.device):
+            _lib.check(
+                lib.fca_build_metadata_rows(
+                    ctypes.byref(md.plan),
+                    block_table.data_ptr(),
+                    block_table.stride(0),
+                    block_table.shape[0],
+                    row_table.data_ptr(),
+                    row_group.data_ptr() if row_group is not None else None,
+                    seq_lens.data_ptr(),
+                    md.meta.data_ptr(),
+                    1 if update and same_workspace else 0,
+                    _stream_ptr(block_table.device),
+                )
+            )
+        return md
+    entry = lib.fca_update_metadata if update and same_workspace else lib.fca_build_metadata
+    with on_device(block_table.device):
         _lib.check(
-            lib.fca_build_metadata_rows(
+            entry(
                 ctypes.byref(md.plan),
                 block_table.data_ptr(),
                 block_table.stride(0),
-                block_table.shape[0],
-                row_table.data_ptr(),
-                row_group.data_ptr() if row_group is not None else None,
                 seq_lens.data_ptr(),
                 md.meta.data_ptr(),
-                1 if update and same_workspace else 0,
                 _stream_ptr(block_table.device),
             )
         )
-        return md
-    entry = lib.fca_update_metadata if update and same_workspace else lib.fca_build_metadata
-    _lib.check(
-        entry(
-            ctypes.byref(md.plan),
-            block_table.data_ptr(),
-            block_table.stride(0),
-            seq_lens.data_ptr(),
-            md.meta.data_ptr(),
-            _stream_ptr(block_table.device),
-        )
-    )
     return md

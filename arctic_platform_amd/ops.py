@@ -19,8 +19,8 @@ import ctypes
 import torch
 
 from . import _lib
-from .cache import check_block_scales, on_device
-from .forest import ForestMetadata, _stream_ptr
+from .cache import check_block_scales
+from .forest import ForestMetadata, _stream_ptr, on_device
 from .kv_layout import BLOCK_SIZE
 
 
@@ -213,11 +213,13 @@ def merge_partials(meta: ForestMetadata, q_like, out=None, return_lse=True, out_
     lib = _lib.load_library()
     out, code = _out_args(q_like, meta, out, out_dtype)
     lse = torch.empty(meta.plan.num_seqs, meta.plan.num_q_heads, dtype=torch.float32, device=out.device) if return_lse else None
-    _lib.check(
-        lib.fca_merge_dtype(
-            ctypes.byref(meta.plan), _lib.FCA_FP8_E4M3_BLOCK if meta.block_scaled else _lib.FCA_BF16, meta.meta.data_ptr(), meta.partial_out.data_ptr(), meta.partial_lse.data_ptr(),
-            out.data_ptr(), out.stride(0), out.stride(1), code, lse.data_ptr() if lse is not None else None,
-            _stream_ptr(out.device),
+    with on_device(out.device):
+        _lib.check(
+            lib.fca_merge_dtype(
+                ctypes.byref(meta.plan), _lib.FCA_FP8_E4M3_BLOCK if meta.block_scaled else _lib.FCA_BF16, meta.meta.data_ptr(),
+                meta.partial_out.data_ptr(), meta.partial_lse.data_ptr(),
+                out.data_ptr(), out.stride(0), out.stride(1), code, lse.data_ptr() if lse is not None else None,
+                _stream_ptr(out.device),
+            )
         )
-    )
     return (out, lse) if return_lse else out

@@ -23,6 +23,7 @@ import numpy as np
 import torch
 
 from . import _lib
+from .forest import on_device
 from .split_attention import SplitLayout, _stream_ptr
 
 
@@ -121,12 +122,13 @@ def _gather(src, index, num_rows):
     if src.shape[0] == 0:  # nothing to take rows from: every index is "none"
         return torch.zeros((num_rows, src.shape[1]), dtype=src.dtype, device=src.device)
     out = torch.empty((num_rows, src.shape[1]), dtype=src.dtype, device=src.device)
-    _lib.check(
-        _lib.load_library().fca_gather_rows(
-            src.data_ptr(), src.stride(0) * src.element_size(), index.data_ptr(), num_rows, src.shape[1] * src.element_size(),
-            out.data_ptr(), out.stride(0) * out.element_size(), _stream_ptr(src.device),
+    with on_device(src.device):
+        _lib.check(
+            _lib.load_library().fca_gather_rows(
+                src.data_ptr(), src.stride(0) * src.element_size(), index.data_ptr(), num_rows, src.shape[1] * src.element_size(),
+                out.data_ptr(), out.stride(0) * out.element_size(), _stream_ptr(src.device),
+            )
         )
-    )
     return out
 
 
@@ -140,12 +142,13 @@ def _sum_copies(src, offsets, rows, num_dst):
     if src.shape[1] % 8:
         raise ValueError("a row must hold a multiple of 8 values")
     out = torch.empty((num_dst, src.shape[1]), dtype=src.dtype, device=src.device)
-    _lib.check(
-        _lib.load_library().fca_sum_rows(
-            src.data_ptr(), src.stride(0) * src.element_size(), offsets.data_ptr(), rows.data_ptr(), num_dst, src.shape[1], code,
-            out.data_ptr(), out.stride(0) * out.element_size(), _stream_ptr(src.device),
+    with on_device(src.device):
+        _lib.check(
+            _lib.load_library().fca_sum_rows(
+                src.data_ptr(), src.stride(0) * src.element_size(), offsets.data_ptr(), rows.data_ptr(), num_dst, src.shape[1], code,
+                out.data_ptr(), out.stride(0) * out.element_size(), _stream_ptr(src.device),
+            )
         )
-    )
     return out
 
 

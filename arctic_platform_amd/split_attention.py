@@ -22,6 +22,7 @@ import numpy as np
 import torch
 
 from . import _lib
+from .forest import on_device
 
 
 def _stream_ptr(device) -> int:
@@ -198,13 +199,14 @@ def split_attention_forward(q, k, v, layout: SplitLayout, scale: float, out=None
     lse = torch.empty((q.shape[1], 32 * layout.num_tiles), dtype=torch.float32, device=q.device)
     if t == 0:
         return out, lse
-    _lib.check(
-        _lib.load_library().fca_split_attention_forward(
-            ctypes.byref(plan), q.data_ptr(), q.stride(0), k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0),
-            layout.dev.data_ptr(), float(scale), layout.scratch(plan, False).data_ptr(), out.data_ptr(), out.stride(0),
-            lse.data_ptr(), _stream_ptr(q.device),
+    with on_device(q.device):
+        _lib.check(
+            _lib.load_library().fca_split_attention_forward(
+                ctypes.byref(plan), q.data_ptr(), q.stride(0), k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0),
+                layout.dev.data_ptr(), float(scale), layout.scratch(plan, False).data_ptr(), out.data_ptr(), out.stride(0),
+                lse.data_ptr(), _stream_ptr(q.device),
+            )
         )
-    )
     return out, lse
 
 
@@ -225,14 +227,15 @@ def split_attention_backward(dout, q, k, v, out, lse, layout: SplitLayout, scale
         _check_rows(name, x, t)
     if t == 0:
         return dq, dk, dv
-    _lib.check(
-        _lib.load_library().fca_split_attention_backward(
-            ctypes.byref(plan), q.data_ptr(), q.stride(0), k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0),
-            out.data_ptr(), out.stride(0), dout.data_ptr(), dout.stride(0), lse.data_ptr(), layout.dev.data_ptr(),
-            float(scale), layout.scratch(plan, True).data_ptr(), dq.data_ptr(), dq.stride(0), dk.data_ptr(), dk.stride(0),
-            dv.data_ptr(), dv.stride(0), _stream_ptr(q.device),
+    with on_device(q.device):
+        _lib.check(
+            _lib.load_library().fca_split_attention_backward(
+                ctypes.byref(plan), q.data_ptr(), q.stride(0), k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0),
+                out.data_ptr(), out.stride(0), dout.data_ptr(), dout.stride(0), lse.data_ptr(), layout.dev.data_ptr(),
+                float(scale), layout.scratch(plan, True).data_ptr(), dq.data_ptr(), dq.stride(0), dk.data_ptr(), dk.stride(0),
+                dv.data_ptr(), dv.stride(0), _stream_ptr(q.device),
+            )
         )
-    )
     return dq, dk, dv
 
 
