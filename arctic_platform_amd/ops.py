@@ -102,6 +102,8 @@ def _out_args(q, meta, out, out_dtype):
         code = _lib.FCA_F32
     else:
         raise TypeError("out must be bfloat16 or float32")
+    if out.device != q.device:
+        raise ValueError(f"out is on {out.device}, q on {q.device}")
     if out.shape != shape or out.stride(2) != 1:
         raise ValueError("out must be [num_seqs, num_q_heads, head_dim] with contiguous head_dim")
     return out, code
@@ -153,6 +155,8 @@ def forest_cascade_decode_static(
     out, code = _out_args(q, meta, out, None)
     if lse is not None and (lse.dtype != torch.float32 or lse.shape != (meta.plan.num_seqs, meta.plan.num_q_heads) or not lse.is_contiguous()):
         raise ValueError("lse must be a contiguous fp32 tensor [num_seqs, num_q_heads]")
+    if lse is not None and lse.device != q.device:
+        raise ValueError(f"lse is on {lse.device}, q on {q.device}")
     with on_device(q.device):
         _lib.check(
             lib.fca_decode_step_static(

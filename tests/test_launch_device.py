@@ -99,3 +99,22 @@ def test_the_trainers_operators(library):
     names = [n for n, _ in library.launched]
     assert "fca_split_attention_forward" in names and "fca_split_attention_backward" in names and "fca_gather_rows" in names and "fca_sum_rows" in names
     assert all(device == torch.device("cpu") for _, device in library.launched), library.launched
+
+
+def test_outputs_on_another_device_are_refused(library):
+    """(A host tensor's address would reach the kernel.)"""
+    table, lens = torch.zeros(2, 4, dtype=torch.int32), torch.tensor([20, 30], dtype=torch.int32)
+    md = forest.build_forest_metadata(table, lens, num_q_heads=4, num_kv_heads=2, head_dim=64)
+    q, elsewhere = torch.zeros(2, 4, 64, dtype=torch.bfloat16), torch.zeros(2, 4, 64, dtype=torch.bfloat16, device="meta")
+    fp8 = torch.zeros(kv_cache_shape(4, 16, 2, 64), dtype=torch.uint8).view(torch.float8_e4m3fn)
+    library.launched = []
+    for kw in (dict(), dict(block_scales=torch.ones(block_scales_shape(4, 2)))):
+        with pytest.raises(ValueError, match="out is on meta"):
+            ops.forest_cascade_decode(q, fp8, md, 0.1, out=elsewhere, **kw)
+        with pytest.raises(ValueError, match="out is on meta"):
+            ops.forest_cascade_decode_static(q, fp8, md, 0.1, out=elsewhere, **kw)
+        with pytest.raises(ValueError, match="lse is on meta"):
+            ops.forest_cascade_decode_static(q, fp8, md, 0.1, out=torch.zeros_like(q), lse=torch.zeros(2, 4, device="meta"), **kw)
+    with pytest.raises(ValueError, match="out is on meta"):
+        ops.merge_partials(md, q, out=elsewhere)
+    assert not library.launched
