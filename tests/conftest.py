@@ -93,3 +93,25 @@ def gpu(request):
 
     _lib.load_library()  # fails loudly if the HIP library was not built
     return torch.device("cuda:0")
+
+
+# Test files whose expected values are sums of torch's own on the GPU, compared bit for bit.  index_add_ adds
+# through atomics there, in an order that changes from run to run, unless torch is asked for its ordered
+# algorithms: then rows are added one after the other, as on the CPU.
+ORDERED_SUMS = ("test_zw_reconstruct",)
+
+
+@pytest.fixture(autouse=True)
+def _ordered_sums(request):
+    if request.module.__name__.rpartition(".")[2] not in ORDERED_SUMS:
+        yield
+        return
+    import torch
+
+    before = torch.are_deterministic_algorithms_enabled(), torch.is_deterministic_algorithms_warn_only_enabled()
+    fill = torch.utils.deterministic.fill_uninitialized_memory
+    torch.use_deterministic_algorithms(True)
+    torch.utils.deterministic.fill_uninitialized_memory = False  # (what the operators under test allocate stays as it is)
+    yield
+    torch.use_deterministic_algorithms(before[0], warn_only=before[1])
+    torch.utils.deterministic.fill_uninitialized_memory = fill
