@@ -89,12 +89,15 @@ __device__ inline V without_nans(V raw, int& found) {
 // of their own next to that of the exponentials: the largest log2(p) + log2(s_v) the row has met.
 // The largest weight is then about 2^kWeightBits; one 2^-21 of it still has 11 bits, and what is lost
 // of a smaller one is below 2^-32 of the largest, whatever the scales of the blocks are.  Measured
-// against bf16 weights with one reference: 0 to 3 % of a call (verify steps 52.5 -> 53.9 us the most).
+// against bf16 weights with one reference: 0 to 4 % of a call (verify steps 52.4 -> 54.7 us the most).
 constexpr float kWeightBits = 7.f;  // + kRescaleSlack = 15: a half ends at 65504
 struct RowState {
-  float m, w;  // references (log2 domain): of the scaled scores, of those plus log2 of the V scale
-  float g;     // weight = exp2(score - m) * V scale * g
-  float l;     // running sum of exp2(score - m)
+  float m;  // reference of the scaled scores (log2 domain)
+  float u;  // that of the weights: largest (score - m) + log2(V scale).  (Relative to m, and from the fused
+            // multiply-add the exponentials take: scores far beyond 2^24 would leave nothing of a V scale's log2
+            // added to them, and their rounding alone moves the exponent of a weight by more than a half holds.)
+  float g;  // 2^(kWeightBits - u): weight = exp2(score - m) * V scale * g
+  float l;  // running sum of exp2(score - m)
 };
 __device__ inline RowState empty_row() { return RowState{-INFINITY, -INFINITY, 1.f, 0.f}; }
 // log2 of a V scale, kept where the writer's scales are: the factor g stays a normal number.
@@ -117,20 +120,29 @@ __device__ inline void weigh_tile(RowState& row, bool first, f32x16 sr, const fl
     mx[blk] = sr[8 * blk];
 #pragma unroll
     for (int r = 1; r < 8; ++r) mx[blk] = fmaxf(mx[blk], sr[8 * blk + r]);
-    mx[blk] *= ks[blk];  // (the scales are positive, so the maximum of the scaled scores is a scaled maximum)
   }
-  float mtile = fmaxf(mx[0], mx[1]), wtile = fmaxf(mx[0] + lv[0], mx[1] + lv[1]);
+  // (the scales are positive, so the maximum of the scaled scores is a scaled maximum)
+  float mtile = fmaxf(mx[0] * ks[0], mx[1] * ks[1]);
   mtile = fmaxf(mtile, other_half(mtile));
-  wtile = fmaxf(wtile, other_half(wtile));
+  auto largest_weight = [&]() {
+    const float x = fmaxf(__builtin_fmaf(mx[0], ks[0], -row.m) + lv[0], __builtin_fmaf(mx[1], ks[1], -row.m) + lv[1]);
+    return fmaxf(x, other_half(x));
+  };
   // The references move (and sum and accumulators are rescaled) only when a maximum rises more than
-  // kRescaleSlack above its own.
-  if (first) row.m = mtile, row.w = wtile, row.g = fast_exp2(mtile - wtile + kWeightBits);
-  if (__ballot(mtile > row.m + kRescaleSlack || wtile > row.w + kRescaleSlack) != 0) {
-    const float m_new = fmaxf(row.m, mtile), w_new = fmaxf(row.w, wtile);
-    const float alpha = fast_exp2(row.w - w_new);
-    row.l *= fast_exp2(row.m - m_new);
-    row.m = m_new, row.w = w_new;
-    row.g = fast_exp2(m_new - w_new + kWeightBits);
+  // kRescaleSlack above its own.  (That a lane looks at its half of the tile's weights first, and at the
+  // other's where it has to, costs the wide kernels scratch: verify steps 69 us instead of 54.7.)
+  if (first) row.m = mtile;
+  float utile = largest_weight();
+  if (first) row.u = utile, row.g = fast_exp2(kWeightBits - utile);
+  if (__ballot(mtile > row.m + kRescaleSlack || utile > row.u + kRescaleSlack) != 0) {
+    const float drop = row.m - fmaxf(row.m, mtile);
+    row.m = fmaxf(row.m, mtile);
+    utile = largest_weight();
+    const float u_new = fmaxf(row.u + drop, utile);
+    const float alpha = fast_exp2(row.u + drop - u_new);
+    row.l *= fast_exp2(drop);
+    row.u = u_new;
+    row.g = fast_exp2(kWeightBits - u_new);
 #pragma unroll
     for (int db = 0; db < NDB; ++db)
 #pragma unroll

@@ -104,3 +104,36 @@ def test_many_small_weights_beside_a_large_one(gpu, d, rows):
     out, lse = forest_cascade_decode(q.to(gpu), cache.to(gpu), md, scale, block_scales=scales.to(gpu), out_dtype=torch.float32)
     torch.cuda.synchronize()
     _check(out, lse, q, cache, scales, table, [n], scale)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("d,rows", [(64, 32), (64, 64), (128, 32), (128, 64), (256, 32)])
+@pytest.mark.parametrize("power", [20, 24, 27, 29])
+def test_scores_far_beyond_their_rounding(gpu, d, rows, power):
+    """Scores of about 2^power, exact by construction and the same for three tokens of a sequence (one in each of three
+    blocks, their V scales far apart), half as large for the others: the output is the mean of three rows."""
+    from arctic_platform_amd import build_forest_metadata, forest_cascade_decode
+
+    hq, hkv, n = 4, 1, 150
+    g = torch.Generator().manual_seed(d + power)
+    nb = (n + 15) // 16
+    k, v = torch.zeros(nb, 16, hkv, d), torch.randn(nb, 16, hkv, d, generator=g)
+    k[:, :, :, 0], top = 0.5, [5, 70, 145]
+    for t in top:
+        k[t // 16, t % 16, :, 0] = 1.0
+    v = v * torch.exp2(torch.randint(-30, 31, (nb, 1, 1, 1), generator=g).float())
+    cache, scales = quantize_blocks(k, v)
+    scales[..., 0], raw = 2.0**-8, cache.view(torch.uint8)[0].view(nb, hkv, d // 16, 16, 16)
+    raw[:, :, 0, :, 0] = torch.tensor([0.5, 1.0]).mul(256).to(torch.float8_e4m3fn).view(torch.uint8)[(k[:, :, 0, 0] == 1).long()][:, None]
+    table = torch.arange(nb, dtype=torch.int32).view(1, -1)
+    q = torch.zeros(1, hq, d)
+    q[..., 0] = 1.1015625 * 2.0**power  # (a bf16 number)
+    md = build_forest_metadata(table.to(gpu), torch.tensor([n], dtype=torch.int32).to(gpu), num_q_heads=hq, num_kv_heads=hkv, head_dim=d, chunk_tokens=64, rows_per_item=rows)
+    out, lse = forest_cascade_decode(q.bfloat16().to(gpu), cache.to(gpu), md, 1.0, block_scales=scales.to(gpu), out_dtype=torch.float32)
+    torch.cuda.synchronize()
+    values = oracle.token_rows(cache, scales, torch.tensor(top), d)[1][:, 0]
+    want, weight = values.mean(dim=0), values.abs().mean(dim=0)
+    # a third each, exactly (but for 2^-22 of exp2); weights and partial rows are halves, 2^-11 of each
+    tol = weight * (2 * 2.0**-11 + 2.0**-18) + weight.max() * 2.0**-20
+    assert ((out.cpu().double()[0] - want).abs() <= tol).all()
+    assert ((lse.cpu().double() - 1.1015625 * 2.0**power).abs() <= 2.0 ** (power - 22) + 2).all()
