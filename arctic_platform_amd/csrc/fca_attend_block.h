@@ -100,8 +100,9 @@ struct RowState {
   float l;  // running sum of exp2(score - m)
 };
 __device__ inline RowState empty_row() { return RowState{-INFINITY, -INFINITY, 1.f, 0.f}; }
-// log2 of a V scale, kept where the writer's scales are: the factor g stays a normal number.
-__device__ inline float scale_log2(float vs) { return fminf(fmaxf(fast_log2(vs), (float)(kScaleExpMin - 127)), (float)(kScaleExpMax - 127)); }
+// log2 of a V scale, kept from where the writer's scales begin (g stays finite; a weight under a smaller scale,
+// in a table of somebody else's, has fewer bits).
+__device__ inline float scale_log2(float vs) { return fmaxf(fast_log2(vs), (float)(kScaleExpMin - 127)); }
 
 // Scores of a tile -> weights, register r holding token 16 * (r / 8) + 8 * h + r % 8 of the tile; ks, vs, lv:
 // K scale (log2 domain), V scale and its log2 of the tile's two blocks.  RAGGED: registers of tokens from

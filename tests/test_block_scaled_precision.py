@@ -137,3 +137,23 @@ def test_scores_far_beyond_their_rounding(gpu, d, rows, power):
     tol = weight * (2 * 2.0**-11 + 2.0**-18) + weight.max() * 2.0**-20
     assert ((out.cpu().double()[0] - want).abs() <= tol).all()
     assert ((lse.cpu().double() - 1.1015625 * 2.0**power).abs() <= 2.0 ** (power - 22) + 2).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("d,rows", [(64, 32), (64, 64), (128, 32), (128, 64), (256, 32)])
+def test_value_scales_beyond_the_writers(gpu, d, rows):
+    """A table of somebody else's: V scales of 2^120 to 2^125 on codes small enough that every value is finite."""
+    from arctic_platform_amd import build_forest_metadata, forest_cascade_decode
+
+    hq, hkv, lens, scale = 4, 2, [40, 100, 3], d**-0.5
+    g = torch.Generator().manual_seed(d + rows)
+    q, cache, scales, table = _batch(g, lens, hq, hkv, d, 0.0)
+    raw = cache.view(torch.uint8)
+    raw[1] = torch.randint(0x08, 0x41, raw[1].shape, generator=g, dtype=torch.uint8) | (raw[1] & 0x80)  # magnitudes of 2^-6 to 2.25
+    scales[..., 1] = torch.exp2(torch.randint(120, 126, scales.shape[:2], generator=g).float())
+    md = build_forest_metadata(
+        table.to(gpu), torch.tensor(lens, dtype=torch.int32).to(gpu), num_q_heads=hq, num_kv_heads=hkv, head_dim=d, chunk_tokens=64, rows_per_item=rows
+    )
+    out, lse = forest_cascade_decode(q.to(gpu), cache.to(gpu), md, scale, block_scales=scales.to(gpu), out_dtype=torch.float32)
+    torch.cuda.synchronize()
+    _check(out, lse, q, cache, scales, table, lens, scale)
