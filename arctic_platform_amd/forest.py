@@ -62,7 +62,7 @@ class ForestMetadata:
     # three where that instance exists (head size 128, 32-row items; fca_tensors.tile_buffers).
     # Calls on a bf16 cache, or with another head size or tile height, are not affected.
     fp8_tile_buffers: int = 0
-    # What the partial buffers hold: a prefix_pass, suffix_pass or forest_pass notes here that it attended
+    # What the partial buffers hold: a call that writes them notes here that it attended
     # over a block-scaled cache, and merge_partials merges as forest_cascade_decode does there.
     block_scaled: bool = False
 

@@ -123,6 +123,7 @@ def forest_cascade_decode(
     _check_partials(meta, t)
     out, code = _out_args(q, meta, out, out_dtype or (torch.float32 if t.kv_dtype == _lib.FCA_F32 else None))
     lse = torch.empty(meta.plan.num_seqs, meta.plan.num_q_heads, dtype=torch.float32, device=q.device) if return_lse else None
+    meta.block_scaled = block_scales is not None
     with on_device(q.device):
         _lib.check(
             lib.fca_decode_step(
