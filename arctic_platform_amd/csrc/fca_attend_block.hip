@@ -14,7 +14,7 @@
 // matrix instructions drop products below 2^-13 of the largest one they add.)
 //
 // Memory-bound where the cache is long: 64 x 8 sequences over prompts of 2560 tokens and 512 of their
-// own (32 query heads, 8 KV heads of 128; 913 MB of codes) take 161 us = 5.7 TB/s, a copy of the kernel
+// own (32 query heads, 8 KV heads of 128; 913 MB of codes) take 163 us = 5.6 TB/s, a copy of the kernel
 // that only loads 153; one sequence of 131071 tokens 46 us = 5.9 TB/s.  Latency-bound where it is short:
 // one sequence of 300 tokens takes 8.4 us, five dependent trips to memory from the header to the rows.
 #include <hip/hip_ext.h>

@@ -15,8 +15,8 @@
 // everyone has finished with the tile before, whose slot the next request refills.
 //
 // Measured (32 query heads, 8 KV heads of 128): 16 x 6 sequences of four query tokens over 1500 + 400
-// tokens 46 us; 8 x 16 over 32768 + 2176 tokens 237 us = 4.7 TB/s, of which the partial rows are 20 (only
-// loading takes 187); 16 query heads on 2 KV heads of 256, 32 x 8 over 2560 + 512 tokens, 67 us.  What
+// tokens 48 us; 8 x 16 over 32768 + 2176 tokens 240 us = 4.7 TB/s, of which the partial rows are 20 (only
+// loading takes 187); 16 query heads on 2 KV heads of 256, 32 x 8 over 2560 + 512 tokens, 69 us.  What
 // bounds it: a wave issues for about 1100 cycles a tile (250 vector and 16 matrix instructions), two
 // share a SIMD and a tile takes a workgroup 0.93 us; an item adds 1 us, the start of a launch 6 to 8
 // (header, records, block ids and query rows are dependent trips to memory, all workgroups at once).

@@ -457,8 +457,9 @@ hipError_t launch_append_block(const BlockCacheParams& p, hipStream_t stream) {
   if (p.num_tokens == 0) return hipSuccess;
   // Windows: at most 512 of them up to their largest size; KV heads: as many groups as bring the launch
   // to 512 workgroups; waves: one for each two tiles of a workgroup, 4 to 8.  Few large workgroups
-  // look at all the slots: 8191 tokens of 8 heads take 17 us, with 1024 workgroups of 4 waves 21, with
-  // twice as many windows 26; 8 tokens take 4.4 (an empty launch: 2.5), 512 tokens of 512 blocks 9.2.
+  // look at all the slots: 8191 tokens of 8 heads take 16.5 us (comparing with all blocks of a window it was
+  // 17.5, and with 1024 workgroups of 4 waves 21, with twice as many windows 26); 8 tokens take 4.7 (an
+  // empty launch: 2.5), 512 tokens of 512 blocks 9.4.
   int window = 1;
   while (window < kMaxWindow && (p.num_tokens + window - 1) / window > 512) window *= 2;
   const int windows = (p.num_tokens + window - 1) / window;

@@ -19,7 +19,6 @@ CLANG = "/opt/rocm/lib/llvm/bin/clang++"
 
 _LDS_HELPERS = """__device__ inline unsigned lds_address(const void* p) { return emu::lds_address(p); }
 __device__ inline void load_to_lds16(const void* src, unsigned lds_slot) { emu::dma_to_lds(src, lds_slot, 16); }
-__device__ inline void stream_to_lds16(const void* src, unsigned lds_slot) { emu::streamed_bytes += 16; emu::dma_to_lds(src, lds_slot, 16); }
 template <int PIECES, bool STREAM>
 __device__ inline void block_to_lds(const char* block, int lane_off, unsigned lds) {
   for (int j = 0; j < PIECES; ++j) {
